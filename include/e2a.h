@@ -365,6 +365,30 @@ int e2a_node_map_fwd(const float* pos, int64_t n_nodes, const double* j1, const 
 int e2a_node_map_bwd(const float* pos, const float* dA, int64_t n_nodes, const double* j1, const double* j2,
                      const int32_t* sel, const double* cg, const int32_t* row_perm, float* dpos, void* stream);
 
+/* ------------------------------------------------------------------------------------------ */
+/* Layer norm over rows of W values with an optional SiLU, for training (nn.LayerNorm, nn.SiLU in  */
+/* RadialProfile and SO3_Linear2Scalar_e2former, module_utils.py:2151-2178, 2240-2274):            */
+/*   xh = (x - mean) rstd,  z = gamma xh + beta,  y = act(z)      act: 0 none, 1 SiLU              */
+/* dtype of x, y and every row tensor: 0 fp32, 1 bf16, 2 fp16; gamma / beta fp32 or NULL (1 / 0).  */
+/* Rows of x, dy and u have the strides ldx, lddy, ldu (elements, >= 0); outputs are contiguous.    */
+/* mean / rstd [rows] fp32 are written by the forward and read by the backward.                     */
+/* Backward: dx (may be NULL), dgamma / dbeta [W] fp32 (may be NULL; with both NULL no workspace).  */
+/* Second order, from the cotangents u of dx and p / q [W] of dgamma / dbeta (p, q may be NULL):     */
+/* d_dy and dx are the gradients of <dx,u> + <dgamma,p> + <dbeta,q> in dy and x, dgamma / dbeta (may */
+/* be NULL) those in gamma and beta.  Column sums in row order, no atomics.                          */
+/* ------------------------------------------------------------------------------------------ */
+int e2a_layer_norm_fwd(const void* x, int64_t ldx, int dtype, const float* gamma, const float* beta, int64_t rows,
+                       int64_t W, float eps, int act, void* y, float* mean, float* rstd, void* stream);
+size_t e2a_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t W);
+int e2a_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, int dtype, const float* gamma,
+                       const float* beta, const float* mean, const float* rstd, int64_t rows, int64_t W, int act,
+                       void* dx, float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes, void* stream);
+size_t e2a_layer_norm_bwd2_workspace_bytes(int64_t rows, int64_t W);
+int e2a_layer_norm_bwd2(const void* x, int64_t ldx, const void* dy, int64_t lddy, const void* u, int64_t ldu, int dtype,
+                        const float* gamma, const float* beta, const float* mean, const float* rstd, const float* p,
+                        const float* q, int64_t rows, int64_t W, int act, void* d_dy, void* dx, float* dgamma,
+                        float* dbeta, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -82,6 +82,11 @@ SIGNATURES = {
                                    I64, P, P, P, P, SZ, P]),
     "e2a_attn_bwd_softmax_logits": (I32, [P, P, P, I64, P, P, P, P, P, I64, I64, I64, I32, I32, I32, P, P, P, P, P,
                                           P, P, P, I64, P, P, P, P]),
+    "e2a_layer_norm_fwd": (I32, [P, I64, I32, P, P, I64, I64, F32, I32, P, P, P, P]),
+    "e2a_layer_norm_bwd_workspace_bytes": (SZ, [I64, I64]),
+    "e2a_layer_norm_bwd": (I32, [P, I64, P, I64, I32, P, P, P, P, I64, I64, I32, P, P, P, P, SZ, P]),
+    "e2a_layer_norm_bwd2_workspace_bytes": (SZ, [I64, I64]),
+    "e2a_layer_norm_bwd2": (I32, [P, I64, P, I64, P, I64, I32, P, P, P, P, P, P, I64, I64, I32, P, P, P, P, P, SZ, P]),
     "e2a_attn_bwd_dk": (I32, [P, P, P, P, P, P, I64, I64, I64, I32, I32, I32, P, P]),
 }
 
