@@ -180,9 +180,9 @@ def prepare(case, seed):
 
 # ------------------------------------------------------------------------------------------------
 # 8-bit moments, in elementary operations.  A block of 256 values shares the power of two of its largest
-# magnitude; a value over it is a small float of 4 exponent bits and 3 (signed first moment) or 4 (square
-# root of the second moment) fraction bits, rounded up with the probability that a fixed sequence over
-# elements and steps gives.
+# magnitude (the next one where rounding up could pass the largest code); a value over it is a small float of
+# 4 exponent bits and 3 (signed first moment) or 4 (square root of the second moment) fraction bits, rounded up
+# with the probability that a fixed sequence over elements and steps gives.
 # ------------------------------------------------------------------------------------------------
 # odd 32-bit fractions of the powers of the root of x^5 = x + 1: additive sequences with independent steps
 _INDEX_STEP = (0xDB4F0B91, 0xA0F2EC75)
@@ -197,7 +197,7 @@ def _dither(index, step, which):
 
 def _pack(x, dither, fraction):
     mag = x.abs()
-    b = (mag.amax(1, keepdim=True).view(torch.int32) >> 23).clamp(27, 253)
+    b = ((mag.amax(1, keepdim=True).view(torch.int32) + (1 << (23 - fraction))) >> 23).clamp(27, 253)
     z = mag * ((254 - b) << 23).view(torch.float32) * 2.0 ** -112
     top = 127 if fraction == 3 else 255
     code = ((z.view(torch.int32) + dither) >> (23 - fraction)).clamp(max=top)
