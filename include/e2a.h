@@ -389,6 +389,41 @@ int e2a_layer_norm_bwd2(const void* x, int64_t ldx, const void* dy, int64_t lddy
                         const float* q, int64_t rows, int64_t W, int act, void* d_dy, void* dx, float* dgamma,
                         float* dbeta, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------ */
+/* The optimiser's step over many tensors (no reference kernel).  Tables of tensors are HOST arrays */
+/* of device addresses and sizes, read before the call returns; dtype 0 fp32, 1 bf16, 2 fp16 for     */
+/* parameters and gradients.                                                                        */
+/*                                                                                                  */
+/* Global norm: e2a_sum_squares writes partial sums (64 bits) of all values' squares to the          */
+/* workspace (e2a_grad_norm_workspace_bytes) and their number to the host; tensors of another type    */
+/* follow by further calls on the rest of the workspace.  e2a_norm_of_squares adds them up in order   */
+/* and writes the root.                                                                             */
+/*                                                                                                  */
+/* e2a_adamw_step: per tensor j with t = ++step[slots[j]] (int32, device),                            */
+/*   g = grad min(1, max_norm / (grad_norm + 1e-6))   (grad_norm device fp32, or NULL: no clipping)   */
+/*   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2                                      */
+/*   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)         */
+/* in fp32, p rounded once to its type.  Unless *grad_norm is finite nothing is changed, step          */
+/* included.  lr_device (fp32, may be NULL) takes lr's place.  The moments are flat: tensor j's start   */
+/* at element state_offset[j], a multiple of 256, in order; slots rise too.  state_bits 32: fp32.      */
+/* state_bits 8: one byte an element and, per 256 of them, one scale byte: x = y 2^(scale - 127) with   */
+/* y a small float, m: sign, 4 exponent, 3 fraction bits; sqrt(v): 4 exponent, 4 fraction bits; exponent */
+/* 15 stands for [1, 2), 0 for the subnormals; scale 255 for a block of NaN.  e2a_moments_unpack gives   */
+/* m and v of n elements as fp32.  Tensors that overlap a parameter are refused (E2A_ERR_ARG).          */
+/* ------------------------------------------------------------------------------------------ */
+size_t e2a_grad_norm_workspace_bytes(int64_t n_tensors);
+int e2a_sum_squares(const uint64_t* tensors, const int64_t* numel, int64_t n_tensors, int dtype, void* workspace,
+                    size_t workspace_bytes, int64_t* n_partials, void* stream);
+int e2a_norm_of_squares(const void* partials, int64_t n_partials, float* norm, void* stream);
+size_t e2a_adamw_workspace_bytes(int64_t n_tensors);
+int e2a_adamw_step(const uint64_t* params, const uint64_t* grads, const int64_t* numel, const int64_t* state_offset,
+                   const int32_t* slots, int64_t n_tensors, int dtype, int state_bits, void* exp_avg, void* exp_avg_sq,
+                   uint8_t* exp_avg_scale, uint8_t* exp_avg_sq_scale, int64_t state_elements, int32_t* step, double lr,
+                   const float* lr_device, double beta1, double beta2, double eps, double weight_decay,
+                   const float* grad_norm, double max_norm, void* workspace, size_t workspace_bytes, void* stream);
+int e2a_moments_unpack(const uint8_t* exp_avg, const uint8_t* exp_avg_sq, const uint8_t* exp_avg_scale,
+                       const uint8_t* exp_avg_sq_scale, int64_t n, float* out_avg, float* out_avg_sq, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,7 @@ I64 = ctypes.c_int64
 I32 = ctypes.c_int
 U64 = ctypes.c_uint64
 F32 = ctypes.c_float
+F64 = ctypes.c_double
 SZ = ctypes.c_size_t
 
 # name -> (restype, argtypes); mirrors include/e2a.h
@@ -87,6 +88,13 @@ SIGNATURES = {
     "e2a_layer_norm_bwd": (I32, [P, I64, P, I64, I32, P, P, P, P, I64, I64, I32, P, P, P, P, SZ, P]),
     "e2a_layer_norm_bwd2_workspace_bytes": (SZ, [I64, I64]),
     "e2a_layer_norm_bwd2": (I32, [P, I64, P, I64, P, I64, I32, P, P, P, P, P, P, I64, I64, I32, P, P, P, P, P, SZ, P]),
+    "e2a_grad_norm_workspace_bytes": (SZ, [I64]),
+    "e2a_sum_squares": (I32, [P, P, I64, I32, P, SZ, P, P]),
+    "e2a_norm_of_squares": (I32, [P, I64, P, P]),
+    "e2a_adamw_workspace_bytes": (SZ, [I64]),
+    "e2a_adamw_step": (I32, [P, P, P, P, P, I64, I32, I32, P, P, P, P, I64, P, F64, P, F64, F64, F64, F64, P, F64,
+                             P, SZ, P]),
+    "e2a_moments_unpack": (I32, [P, P, P, P, I64, P, P, P]),
     "e2a_attn_bwd_dk": (I32, [P, P, P, P, P, P, I64, I64, I64, I32, I32, I32, P, P]),
 }
 

@@ -1,0 +1,280 @@
+"""Optimiser of force-loss training: :class:`AdamW` over all of a model's tensors in a few launches, with its
+moments in 32 or 8 bits, and :func:`grad_norm`, the global gradient norm that clips its step.
+
+Nothing here reads the device: the clipping factor, the step counts and the decision to leave out a step whose
+gradients are not finite stay in device memory (the reference's trainer reads a flag back for the latter,
+pipeline/trainer.py:397-414), so a training step can be captured in a CUDA graph.
+"""
+from __future__ import annotations
+
+from array import array
+
+import torch
+
+from . import _lib
+from ._lib import check, ptr, require_cuda, stream_of
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+BLOCK = 256          # elements that share a scale; every tensor's state starts at a multiple
+
+
+def _address(a):
+    return a.buffer_info()[0]
+
+
+def _pointers(tensors):
+    return array("Q", map(torch.Tensor.data_ptr, tensors))
+
+
+def _one_device(tensors, what):
+    devices = set(map(torch.Tensor.get_device, tensors))
+    if len(devices) > 1 or min(devices) < 0:
+        require_cuda(*tensors)
+        raise ValueError(f"{what} are on more than one device")
+    return tensors[0].device
+
+
+def grad_norm(tensors):
+    """The global L2 norm ``sqrt(sum of all squares)`` of ``tensors`` (float32, bfloat16 or float16 on one CUDA
+    device, any shapes) as a 0-dim float32 tensor there: sums in 64 bits, in a fixed order, no host read.  An
+    empty list has norm 0 on the current device."""
+    tensors = list(tensors)
+    dev = _one_device(tensors, "the tensors") if tensors else torch.device("cuda", torch.cuda.current_device())
+    lib = _lib.load()
+    by_type = {}
+    for t in tensors:
+        if t.layout != torch.strided or t.dtype not in _DTYPES:
+            raise TypeError(f"grad_norm takes strided float32, bfloat16 or float16 tensors, got {t.dtype}, {t.layout}")
+        by_type.setdefault(t.dtype, []).append(t.detach().contiguous())
+    with torch.cuda.device(dev):
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        size = sum(lib.e2a_grad_norm_workspace_bytes(len(ts)) for ts in by_type.values())
+        ws = torch.empty(max(size, 8), dtype=torch.uint8, device=dev)
+        done, count = 0, array("q", [0])
+        for dtype, ts in by_type.items():
+            pt, num = _pointers(ts), array("q", map(torch.Tensor.numel, ts))
+            check(lib.e2a_sum_squares(_address(pt), _address(num), len(ts), _DTYPES[dtype], ws.data_ptr() + 8 * done,
+                                      ws.numel() - 8 * done, _address(count), stream_of(dev)), "e2a_sum_squares")
+            done += count[0]
+        check(lib.e2a_norm_of_squares(ptr(ws), done, ptr(norm), stream_of(dev)), "e2a_norm_of_squares")
+    return norm
+
+
+class _Flat:
+    """The state of one parameter group: flat moments, every tensor at a multiple of 256 elements, and a step
+    count per tensor."""
+
+    def __init__(self, params, bits):
+        self.device = _one_device(params, "a group's parameters")
+        self.numel = [p.numel() for p in params]
+        self.offset, end = [], 0
+        for n in self.numel:
+            self.offset.append(end)
+            end += -(-n // BLOCK) * BLOCK
+        self.elements, self.bits = end, bits
+        kind = torch.float32 if bits == 32 else torch.uint8
+        self.buffers = {"step": torch.zeros(len(params), dtype=torch.int32, device=self.device),
+                        "exp_avg": torch.zeros(end, dtype=kind, device=self.device),
+                        "exp_avg_sq": torch.zeros(end, dtype=kind, device=self.device)}
+        if bits == 8:
+            for k in ("exp_avg_scale", "exp_avg_sq_scale"):
+                self.buffers[k] = torch.zeros(end // BLOCK, dtype=torch.uint8, device=self.device)
+
+    def view(self, i, param):
+        """The state of tensor ``i``: views of the flat buffers."""
+        n, o = self.numel[i], self.offset[i]
+        out = {"step": self.buffers["step"][i], "exp_avg": self.buffers["exp_avg"][o:o + n].view(param.shape),
+               "exp_avg_sq": self.buffers["exp_avg_sq"][o:o + n].view(param.shape)}
+        for k in ("exp_avg_scale", "exp_avg_sq_scale"):
+            if k in self.buffers:
+                out[k] = self.buffers[k][o // BLOCK:(o + n + BLOCK - 1) // BLOCK]
+        return out
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) with PyTorch's arguments and update; parameters in float32, bfloat16 or
+    float16, contiguous, the arithmetic in fp32 with one rounding to the parameter's type.
+
+    * ``state_bits``: 32 = fp32 moments; 8 = one byte per element and moment plus one scale byte per 256
+      (see ``csrc/e2a_optim.cu``), rounded so that averages stay unbiased over steps.
+    * ``max_grad_norm``: clip the gradients of each step to this global norm (over all groups) inside the update;
+      the gradients themselves are left as they are.  The norm of the last step is ``last_grad_norm`` (0-dim
+      tensor on the device).  A step whose norm is not finite changes nothing, step counts included.
+    * ``lr`` of a group: a float, or a float32 tensor of one element on the parameters' device, which a captured
+      step reads anew at every replay.
+
+    Parameters without a gradient are left out of a step, each has its own step count.  State entries
+    (``step``, ``exp_avg``, ``exp_avg_sq`` and, in 8 bits, their ``_scale``) are views of one flat buffer per
+    group (:meth:`flat_state`); ``state_dict`` / ``load_state_dict`` keep types and bits."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
+                 max_grad_norm=None):
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits={state_bits!r}: expected 32 or 8")
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise ValueError(f"max_grad_norm={max_grad_norm!r} must be positive")
+        self.state_bits, self.max_grad_norm, self.last_grad_norm = state_bits, max_grad_norm, None
+        self._flat = {}
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        g = self.param_groups[-1]
+        try:
+            b1, b2 = g["betas"]
+            if not (0 <= b1 < 1 and 0 <= b2 < 1 and g["eps"] >= 0 and g["weight_decay"] >= 0):
+                raise ValueError(f"invalid betas {g['betas']}, eps {g['eps']} or weight_decay {g['weight_decay']}")
+            if not isinstance(g["lr"], torch.Tensor) and not g["lr"] >= 0:
+                raise ValueError(f"invalid lr {g['lr']}")
+            if len(set(map(id, g["params"]))) != len(g["params"]):
+                raise ValueError("a parameter appears twice in a group")
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    # -- state -------------------------------------------------------------------------------------
+    def _group_state(self, i):
+        flat = self._flat.get(i)
+        if flat is None:
+            params = self.param_groups[i]["params"]
+            flat = self._flat[i] = _Flat(params, self.state_bits)
+            for k, p in enumerate(params):
+                self.state[p] = flat.view(k, p)
+        return flat
+
+    def flat_state(self, group=0):
+        """The flat buffers of a group: ``step`` [tensors], ``exp_avg`` and ``exp_avg_sq`` [elements] (each tensor
+        from the next multiple of 256 on), in 8 bits also ``exp_avg_scale`` / ``exp_avg_sq_scale``."""
+        return dict(self._group_state(group).buffers)
+
+    def moments(self, group=0):
+        """``(exp_avg, exp_avg_sq)`` of a group as flat fp32 values (the buffers themselves with 32 bits)."""
+        flat = self._group_state(group)
+        b = flat.buffers
+        if flat.bits == 32:
+            return b["exp_avg"], b["exp_avg_sq"]
+        with torch.cuda.device(flat.device):
+            m = torch.empty(flat.elements, dtype=torch.float32, device=flat.device)
+            v = torch.empty_like(m)
+            check(_lib.load().e2a_moments_unpack(ptr(b["exp_avg"]), ptr(b["exp_avg_sq"]), ptr(b["exp_avg_scale"]),
+                                                 ptr(b["exp_avg_sq_scale"]), flat.elements, ptr(m), ptr(v),
+                                                 stream_of(flat.device)), "e2a_moments_unpack")
+        return m, v
+
+    def load_state_dict(self, state_dict):
+        """Restores types and bits as they were saved; a state of other bits or shapes is refused."""
+        groups = state_dict["param_groups"]
+        held = state_dict["state"]
+        wanted = {"step", "exp_avg", "exp_avg_sq"} | (
+            {"exp_avg_scale", "exp_avg_sq_scale"} if self.state_bits == 8 else set())
+        kind = torch.float32 if self.state_bits == 32 else torch.uint8
+        for k, s in held.items():
+            if set(s) != wanted or s["exp_avg"].dtype != kind or s["exp_avg_sq"].dtype != kind:
+                raise ValueError(f"state of parameter {k} is not one of {self.state_bits}-bit moments")
+        pairs = [(i, k, p) for g, mine in zip(groups, self.param_groups)
+                 for k, (i, p) in enumerate(zip(g["params"], mine["params"]))]
+        for i, _, p in pairs:
+            if i in held and (held[i]["exp_avg"].shape != p.shape or held[i]["exp_avg_sq"].shape != p.shape):
+                raise ValueError(f"state of parameter {i} has another shape than the parameter")
+        super().load_state_dict({"state": {}, "param_groups": groups})    # checks and takes the groups
+        self._flat = {}
+        with torch.no_grad():
+            for gi, (g, mine) in enumerate(zip(groups, self.param_groups)):
+                if not any(i in held for i in g["params"]):
+                    continue
+                self._group_state(gi)
+                for i, p in zip(g["params"], mine["params"]):
+                    for key, t in held.get(i, {}).items():
+                        self.state[p][key].copy_(t)
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits, "max_grad_norm": self.max_grad_norm,
+                "last_grad_norm": self.last_grad_norm}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        held, self._flat = self.state, {}
+        for gi, g in enumerate(self.param_groups):      # a copy's state becomes views of its own flat buffers
+            old = {k: held[p] for k, p in enumerate(g["params"]) if p in held}
+            if old:
+                self._group_state(gi)
+                for k, entries in old.items():
+                    for key, t in entries.items():
+                        self.state[g["params"][k]][key].copy_(t)
+
+    # -- the step ----------------------------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work = []
+        for gi, g in enumerate(self.param_groups):
+            params = g["params"]
+            grads = [p.grad for p in params]
+            if any(t is None for t in grads):
+                index = [k for k, t in enumerate(grads) if t is not None]
+                params, grads = [params[k] for k in index], [grads[k] for k in index]
+            else:
+                index = None
+            if grads:
+                work.append((gi, g, params, grads, index))
+        if not work:
+            return loss
+        norm = None
+        if self.max_grad_norm is not None:
+            norm = self.last_grad_norm = grad_norm([t for w in work for t in w[3]])
+        for gi, g, params, grads, index in work:
+            self._step_group(gi, g, params, grads, index, norm)
+        return loss
+
+    def _step_group(self, gi, group, params, grads, index, norm):
+        flat = self._group_state(gi)
+        dev = flat.device
+        if index is None:
+            index = range(len(params))
+        if _one_device(params, "a group's parameters") != dev:
+            raise ValueError("the parameters have moved to another device than their state")
+        if norm is not None and norm.device != dev:
+            norm = norm.to(dev)
+        if not all(map(torch.Tensor.is_contiguous, params)):
+            raise ValueError("AdamW takes contiguous parameters")
+        grads = [t if t.is_contiguous() else t.contiguous() for t in map(_dense, grads)]
+        if list(map(torch.Tensor.numel, params)) != [flat.numel[k] for k in index]:
+            raise ValueError("a parameter has changed its size since its state was made")
+        lr = group["lr"]
+        if isinstance(lr, torch.Tensor) and lr.is_cuda:
+            if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev:
+                raise ValueError("a tensor lr must be one float32 value on the parameters' device")
+        else:
+            lr = float(lr)
+        by_type = {}
+        for k, p, t in zip(index, params, grads):
+            by_type.setdefault(p.dtype, []).append((k, p, t))
+        lib, b = _lib.load(), flat.buffers
+        with torch.cuda.device(dev):
+            for dtype, items in by_type.items():
+                if dtype not in _DTYPES:
+                    raise TypeError(f"AdamW takes float32, bfloat16 or float16 parameters, got {dtype}")
+                pp, pg = _pointers([p for _, p, _ in items]), _pointers([t for _, _, t in items])
+                num = array("q", [flat.numel[k] for k, _, _ in items])
+                off = array("q", [flat.offset[k] for k, _, _ in items])
+                slot = array("i", [k for k, _, _ in items])
+                ws = torch.empty(lib.e2a_adamw_workspace_bytes(len(items)), dtype=torch.uint8, device=dev)
+                tensor_lr = isinstance(lr, torch.Tensor)
+                check(lib.e2a_adamw_step(
+                    _address(pp), _address(pg), _address(num), _address(off), _address(slot), len(items),
+                    _DTYPES[dtype], flat.bits, ptr(b["exp_avg"]), ptr(b["exp_avg_sq"]), ptr(b.get("exp_avg_scale")),
+                    ptr(b.get("exp_avg_sq_scale")), flat.elements, ptr(b["step"]), 0.0 if tensor_lr else lr,
+                    ptr(lr) if tensor_lr else None, float(group["betas"][0]), float(group["betas"][1]),
+                    float(group["eps"]), float(group["weight_decay"]), ptr(norm), float(self.max_grad_norm or 0.0),
+                    ptr(ws), ws.numel(), stream_of(dev)), "e2a_adamw_step")
+        # the kernels write behind autograd's back: saved tensors and caches keyed on versions have to see it
+        torch.autograd.graph.increment_version(params)
+
+
+def _dense(t):
+    if t.layout != torch.strided:
+        raise TypeError("AdamW takes strided gradients")
+    return t
