@@ -214,6 +214,530 @@ __global__ void k_ln_cols_sum(const double* __restrict__ part, int64_t chunks, i
   out[c < W ? c : c - W] = (float)s;
 }
 
+// ------------------------------------------------------------------------------------------------
+// Rows in registers.  A team of TEAM threads holds a row, VEC neighbouring values (16 bytes, or one where the
+// strides or addresses allow no more) V times a thread, and RB rows at a time so that enough loads are in flight.
+// Teams of at most a warp share a CTA of 256 threads and meet only in shuffles; wider rows take a CTA each.
+// ------------------------------------------------------------------------------------------------
+template <typename T, int VEC> struct Pack;
+template <> struct Pack<float, 4> {
+  static __device__ __forceinline__ void load(const float* p, float* v) {
+    const float4 t = ldg4(p);
+    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+  }
+  static __device__ __forceinline__ void store(float* p, const float* v) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+};
+template <typename T, typename T2> struct Pack16 {
+  static __device__ __forceinline__ void load(const T* p, float* v) {
+    const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const T2 h = *reinterpret_cast<const T2*>(&w[i]);
+      v[2 * i] = to_f(h.x);
+      v[2 * i + 1] = to_f(h.y);
+    }
+  }
+  static __device__ __forceinline__ void store(T* p, const float* v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      T2 h;
+      h.x = from_f<T>(v[2 * i]);
+      h.y = from_f<T>(v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <> struct Pack<__nv_bfloat16, 8> : Pack16<__nv_bfloat16, __nv_bfloat162> {};
+template <> struct Pack<__half, 8> : Pack16<__half, __half2> {};
+template <typename T> struct Pack<T, 1> {
+  static __device__ __forceinline__ void load(const T* p, float* v) { v[0] = to_f(p[0]); }
+  static __device__ __forceinline__ void store(T* p, const float* v) { p[0] = from_f<T>(v[0]); }
+};
+
+// fp32 vectors of the affine parameters: VEC at a time in 16-byte loads (they come from fresh or parameter
+// allocations; the host checks), without them the constant.
+template <int VEC>
+__device__ __forceinline__ void load_affine(const float* p, int c, float without, float* v) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = without;
+  } else if (VEC == 1) {
+    v[0] = __ldg(p + c);
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 4) {
+      const float4 t = ldg4(p + c + k);
+      v[k] = t.x; v[k + 1] = t.y; v[k + 2] = t.z; v[k + 3] = t.w;
+    }
+  }
+}
+
+// Sums over a team of N values a thread; every thread of the team gets them.  CTA-wide teams alternate between
+// two halves of `sh`, so one barrier a sum is enough.
+template <int TEAM, int N>
+__device__ __forceinline__ void team_sum(float (&v)[N], float* sh, int& turn) {
+#pragma unroll
+  for (int o = (TEAM < 32 ? TEAM : 32) / 2; o > 0; o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  }
+  if (TEAM > 32) {
+    constexpr int WARPS = TEAM / 32;
+    float* half = sh + turn * WARPS * 5;
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) half[i * WARPS + (threadIdx.x >> 5)] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) s += half[i * WARPS + w];
+      v[i] = s;
+    }
+  }
+}
+
+template <typename T_, int VEC_, int V_, int TEAM_, int RB_>
+struct Shape {
+  using T = T_;
+  static constexpr int VEC = VEC_, V = V_, TEAM = TEAM_, RB = RB_;
+  static constexpr int THREADS = TEAM > 256 ? TEAM : (TEAM > 32 ? TEAM : 256);
+  static constexpr int TEAMS = THREADS / TEAM;   // rows that a CTA holds at a time, times RB
+  static constexpr int N = VEC * V;
+  static constexpr int COLS = N * TEAM;
+};
+
+template <class S>
+__global__ void __launch_bounds__(S::THREADS)
+k_row_fwd(const typename S::T* __restrict__ x, int64_t ldx, Norm n, int64_t rows, float eps,
+          typename S::T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+  using P = Pack<typename S::T, S::VEC>;
+  __shared__ float sh[S::TEAM > 32 ? 2 * 5 * (S::TEAM / 32) : 1];
+  int turn = 0;
+  const int me = threadIdx.x % S::TEAM, team = threadIdx.x / S::TEAM, W = (int)n.W;
+  const float inv = 1.f / W;
+  for (int64_t base = blockIdx.x * (int64_t)(S::TEAMS * S::RB); base < rows;
+       base += gridDim.x * (int64_t)(S::TEAMS * S::RB)) {
+    float v[S::RB][S::N];
+    int64_t row[S::RB];
+#pragma unroll
+    for (int b = 0; b < S::RB; ++b) {
+      row[b] = base + b * S::TEAMS + team;
+#pragma unroll
+      for (int i = 0; i < S::V; ++i) {
+        const int c = (me + S::TEAM * i) * S::VEC;
+        if (row[b] < rows && c < W) {
+          P::load(x + row[b] * ldx + c, v[b] + i * S::VEC);
+        } else {
+#pragma unroll
+          for (int k = 0; k < S::VEC; ++k) v[b][i * S::VEC + k] = 0.f;
+        }
+      }
+    }
+    float mean[S::RB], var[S::RB];
+#pragma unroll
+    for (int b = 0; b < S::RB; ++b) {
+      mean[b] = 0.f;
+#pragma unroll
+      for (int k = 0; k < S::N; ++k) mean[b] += v[b][k];
+    }
+    team_sum<S::TEAM>(mean, sh, turn);
+#pragma unroll
+    for (int b = 0; b < S::RB; ++b) {
+      mean[b] *= inv;
+      var[b] = 0.f;
+#pragma unroll
+      for (int i = 0; i < S::V; ++i) {
+        if ((me + S::TEAM * i) * S::VEC < W) {
+#pragma unroll
+          for (int k = 0; k < S::VEC; ++k) {
+            float& t = v[b][i * S::VEC + k];
+            t -= mean[b];
+            var[b] += t * t;
+          }
+        }
+      }
+    }
+    team_sum<S::TEAM>(var, sh, turn);
+#pragma unroll
+    for (int b = 0; b < S::RB; ++b) {
+      var[b] = 1.f / sqrtf(var[b] * inv + eps);      // rstd
+      if (me == 0 && row[b] < rows) {
+        mean_out[row[b]] = mean[b];
+        rstd_out[row[b]] = var[b];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < S::V; ++i) {
+      const int c = (me + S::TEAM * i) * S::VEC;
+      if (c < W) {
+        float ga[S::VEC], be[S::VEC];
+        load_affine<S::VEC>(n.gamma, c, 1.f, ga);
+        load_affine<S::VEC>(n.beta, c, 0.f, be);
+#pragma unroll
+        for (int b = 0; b < S::RB; ++b) {
+          float o[S::VEC];
+#pragma unroll
+          for (int k = 0; k < S::VEC; ++k)
+            o[k] = activation(v[b][i * S::VEC + k] * var[b] * ga[k] + be[k], n.silu).y;
+          if (row[b] < rows) P::store(y + row[b] * W + c, o);
+        }
+      }
+    }
+  }
+}
+
+// Adds the column sums that the CTA's threads hold to its partial rows part[2][W], and clears them.
+template <class S>
+__device__ __forceinline__ void flush_cols(float (&dw)[S::N], float (&db)[S::N], float* __restrict__ part, int W,
+                                           bool first, float* sh) {
+  const int me = threadIdx.x % S::TEAM;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    float(&d)[S::N] = which ? db : dw;
+    float* out = part + which * W;
+    if (S::TEAM > 32) {
+#pragma unroll
+      for (int i = 0; i < S::V; ++i) {
+#pragma unroll
+        for (int k = 0; k < S::VEC; ++k) {
+          const int c = (me + S::TEAM * i) * S::VEC + k;
+          if (c < W) out[c] = first ? d[i * S::VEC + k] : out[c] + d[i * S::VEC + k];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int o = 16; o >= S::TEAM; o >>= 1) {
+#pragma unroll
+        for (int k = 0; k < S::N; ++k) d[k] += __shfl_xor_sync(0xffffffffu, d[k], o);
+      }
+      constexpr int WARPS = S::THREADS / 32;
+      __syncthreads();
+      if ((threadIdx.x & 31) < S::TEAM) {
+#pragma unroll
+        for (int i = 0; i < S::V; ++i) {
+#pragma unroll
+          for (int k = 0; k < S::VEC; ++k)
+            sh[(threadIdx.x >> 5) * S::COLS + (me + S::TEAM * i) * S::VEC + k] = d[i * S::VEC + k];
+        }
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < W; c += S::THREADS) {
+        float s = first ? 0.f : out[c];
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) s += sh[w * S::COLS + c];
+        out[c] = s;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < S::N; ++k) d[k] = 0.f;
+  }
+}
+
+constexpr int kChain = 128;   // rows that a thread adds up in fp32 before its sums join the partial rows
+
+// part NULL: dx alone; dx NULL: the column sums alone.
+template <class S>
+__global__ void __launch_bounds__(S::THREADS)
+k_row_bwd(const typename S::T* __restrict__ x, int64_t ldx, const typename S::T* __restrict__ g, int64_t ldg, Norm n,
+          const float* __restrict__ mean_in, const float* __restrict__ rstd_in, int64_t rows,
+          typename S::T* __restrict__ dx, float* __restrict__ part) {
+  using P = Pack<typename S::T, S::VEC>;
+  __shared__ float sh[S::TEAM > 32 ? 2 * 5 * (S::TEAM / 32) : (S::THREADS / 32) * S::COLS];
+  int turn = 0;
+  const int me = threadIdx.x % S::TEAM, team = threadIdx.x / S::TEAM, W = (int)n.W;
+  const float inv = 1.f / W;
+  float dw[S::N], db[S::N];
+#pragma unroll
+  for (int k = 0; k < S::N; ++k) dw[k] = db[k] = 0.f;
+  int held = 0;
+  bool first = true;
+  if (part) part += blockIdx.x * (int64_t)(2 * W);
+  for (int64_t base = blockIdx.x * (int64_t)(S::TEAMS * S::RB); base < rows;
+       base += gridDim.x * (int64_t)(S::TEAMS * S::RB)) {
+    float xh[S::RB][S::N], h[S::RB][S::N], rstd[S::RB];
+    int64_t row[S::RB];
+#pragma unroll
+    for (int b = 0; b < S::RB; ++b) {
+      row[b] = base + b * S::TEAMS + team;
+#pragma unroll
+      for (int i = 0; i < S::V; ++i) {
+        const int c = (me + S::TEAM * i) * S::VEC;
+        if (row[b] < rows && c < W) {
+          P::load(x + row[b] * ldx + c, xh[b] + i * S::VEC);
+          P::load(g + row[b] * ldg + c, h[b] + i * S::VEC);
+        } else {
+#pragma unroll
+          for (int k = 0; k < S::VEC; ++k) xh[b][i * S::VEC + k] = h[b][i * S::VEC + k] = 0.f;
+        }
+      }
+    }
+    float sums[2 * S::RB];
+#pragma unroll
+    for (int b = 0; b < S::RB; ++b) {
+      const float mean = row[b] < rows ? mean_in[row[b]] : 0.f;
+      rstd[b] = row[b] < rows ? rstd_in[row[b]] : 0.f;
+      sums[2 * b] = sums[2 * b + 1] = 0.f;
+#pragma unroll
+      for (int k = 0; k < S::N; ++k) xh[b][k] = (xh[b][k] - mean) * rstd[b];
+    }
+#pragma unroll
+    for (int i = 0; i < S::V; ++i) {
+      const int c = (me + S::TEAM * i) * S::VEC;
+      if (c < W) {
+        float ga[S::VEC], be[S::VEC];
+        load_affine<S::VEC>(n.gamma, c, 1.f, ga);
+        load_affine<S::VEC>(n.beta, c, 0.f, be);
+#pragma unroll
+        for (int b = 0; b < S::RB; ++b) {
+#pragma unroll
+          for (int k = 0; k < S::VEC; ++k) {
+            const int e = i * S::VEC + k;
+            const float a = h[b][e] * activation(xh[b][e] * ga[k] + be[k], n.silu).d1;
+            dw[e] += a * xh[b][e];
+            db[e] += a;
+            h[b][e] = a * ga[k];
+            sums[2 * b] += h[b][e];
+            sums[2 * b + 1] += h[b][e] * xh[b][e];
+          }
+        }
+      }
+    }
+    if (dx) {
+      team_sum<S::TEAM>(sums, sh, turn);
+#pragma unroll
+      for (int b = 0; b < S::RB; ++b) {
+        const float m1 = sums[2 * b] * inv, m2 = sums[2 * b + 1] * inv;
+#pragma unroll
+        for (int i = 0; i < S::V; ++i) {
+          const int c = (me + S::TEAM * i) * S::VEC;
+          float o[S::VEC];
+#pragma unroll
+          for (int k = 0; k < S::VEC; ++k) {
+            const int e = i * S::VEC + k;
+            o[k] = rstd[b] * (h[b][e] - m1 - xh[b][e] * m2);
+          }
+          if (row[b] < rows && c < W) P::store(dx + row[b] * W + c, o);
+        }
+      }
+    }
+    held += S::RB;
+    if (part && held >= kChain) {
+      flush_cols<S>(dw, db, part, W, first, sh);
+      first = false;
+      held = 0;
+    }
+  }
+  if (part && (held || first)) flush_cols<S>(dw, db, part, W, first, sh);
+}
+
+template <class S, bool PQ>
+__global__ void __launch_bounds__(S::THREADS)
+k_row_bwd2(const typename S::T* __restrict__ x, int64_t ldx, const typename S::T* __restrict__ g, int64_t ldg,
+           const typename S::T* __restrict__ u, int64_t ldu, Norm n, const float* __restrict__ mean_in,
+           const float* __restrict__ rstd_in, int64_t rows, typename S::T* __restrict__ dg,
+           typename S::T* __restrict__ dx, float* __restrict__ part) {
+  using P = Pack<typename S::T, S::VEC>;
+  __shared__ float sh[S::TEAM > 32 ? 2 * 5 * (S::TEAM / 32) : (S::THREADS / 32) * S::COLS];
+  int turn = 0;
+  const int me = threadIdx.x % S::TEAM, team = threadIdx.x / S::TEAM, W = (int)n.W;
+  const float inv = 1.f / W;
+  float dw[S::N], db[S::N];
+#pragma unroll
+  for (int k = 0; k < S::N; ++k) dw[k] = db[k] = 0.f;
+  int held = 0;
+  bool first = true;
+  if (part) part += blockIdx.x * (int64_t)(2 * W);
+  for (int64_t base = blockIdx.x * (int64_t)S::TEAMS; base < rows; base += gridDim.x * (int64_t)S::TEAMS) {
+    const int64_t row = base + team;
+    const bool in = row < rows;
+    float xh[S::N], gv[S::N], uv[S::N];
+#pragma unroll
+    for (int i = 0; i < S::V; ++i) {
+      const int c = (me + S::TEAM * i) * S::VEC;
+      if (in && c < W) {
+        P::load(x + row * ldx + c, xh + i * S::VEC);
+        P::load(g + row * ldg + c, gv + i * S::VEC);
+        P::load(u + row * ldu + c, uv + i * S::VEC);
+      } else {
+#pragma unroll
+        for (int k = 0; k < S::VEC; ++k) xh[i * S::VEC + k] = gv[i * S::VEC + k] = uv[i * S::VEC + k] = 0.f;
+      }
+    }
+    const float mean = in ? mean_in[row] : 0.f, rstd = in ? rstd_in[row] : 0.f;
+    float s5[5] = {0.f, 0.f, 0.f, 0.f, 0.f};    // u, u xh, h, h xh, h u
+#pragma unroll
+    for (int i = 0; i < S::V; ++i) {
+      const int c = (me + S::TEAM * i) * S::VEC;
+      if (c < W) {
+        float ga[S::VEC], be[S::VEC];
+        load_affine<S::VEC>(n.gamma, c, 1.f, ga);
+        load_affine<S::VEC>(n.beta, c, 0.f, be);
+#pragma unroll
+        for (int k = 0; k < S::VEC; ++k) {
+          const int e = i * S::VEC + k;
+          xh[e] = (xh[e] - mean) * rstd;
+          const float h = gv[e] * activation(xh[e] * ga[k] + be[k], n.silu).d1 * ga[k];
+          s5[0] += uv[e];
+          s5[1] += uv[e] * xh[e];
+          s5[2] += h;
+          s5[3] += h * xh[e];
+          s5[4] += h * uv[e];
+        }
+      }
+    }
+    team_sum<S::TEAM>(s5, sh, turn);
+    const float su = s5[0] * inv, sc = s5[1] * inv, m2 = s5[3] * inv;
+    const float ht = rstd * (s5[4] * inv - s5[2] * inv * su - m2 * sc);
+    float s2[2] = {0.f, 0.f};                   // k, k xh
+#pragma unroll
+    for (int i = 0; i < S::V; ++i) {
+      const int c = (me + S::TEAM * i) * S::VEC;
+      if (c < W) {
+        float ga[S::VEC], be[S::VEC], pc[S::VEC], qc[S::VEC], o[S::VEC];
+        load_affine<S::VEC>(n.gamma, c, 1.f, ga);
+        load_affine<S::VEC>(n.beta, c, 0.f, be);
+        if (PQ) {
+          load_affine<S::VEC>(n.p, c, 0.f, pc);
+          load_affine<S::VEC>(n.q, c, 0.f, qc);
+        }
+#pragma unroll
+        for (int k = 0; k < S::VEC; ++k) {
+          const int e = i * S::VEC + k;
+          const Act a = activation(xh[e] * ga[k] + be[k], n.silu);
+          const float t = rstd * (uv[e] - su - xh[e] * sc);
+          const float v = PQ ? ga[k] * t + pc[k] * xh[e] + qc[k] : ga[k] * t;
+          const float ag = gv[e] * a.d1, er = gv[e] * a.d2 * v;
+          o[k] = a.d1 * v;
+          dw[e] += ag * t + er * xh[e];
+          db[e] += er;
+          float kk = er * ga[k] - rstd * (uv[e] * m2 + ag * ga[k] * sc);
+          if (PQ) kk += ag * pc[k];
+          uv[e] = kk;
+          s2[0] += kk;
+          s2[1] += kk * xh[e];
+        }
+        if (in) P::store(dg + row * W + c, o);
+      }
+    }
+    team_sum<S::TEAM>(s2, sh, turn);
+    const float k1 = s2[0] * inv, k2 = s2[1] * inv + ht;
+#pragma unroll
+    for (int i = 0; i < S::V; ++i) {
+      const int c = (me + S::TEAM * i) * S::VEC;
+      float o[S::VEC];
+#pragma unroll
+      for (int k = 0; k < S::VEC; ++k) {
+        const int e = i * S::VEC + k;
+        o[k] = rstd * (uv[e] - k1 - xh[e] * k2);
+      }
+      if (in && c < W) P::store(dx + row * W + c, o);
+    }
+    if (part && ++held == kChain) {
+      flush_cols<S>(dw, db, part, W, first, sh);
+      first = false;
+      held = 0;
+    }
+  }
+  if (part && (held || first)) flush_cols<S>(dw, db, part, W, first, sh);
+}
+
+// Column c of the partial rows, added up in row order by 32 threads in 64 bits.
+__global__ void __launch_bounds__(1024)
+k_part_sum(const float* __restrict__ part, int n_part, int W, float* __restrict__ dw, float* __restrict__ db) {
+  __shared__ double sh[32][33];
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  double s = 0.;
+  if (c < 2 * W) {
+#pragma unroll 4
+    for (int i = threadIdx.y; i < n_part; i += 32) s += part[(int64_t)i * 2 * W + c];
+  }
+  sh[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  s = sh[threadIdx.x][threadIdx.y];
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int col = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && col < 2 * W) {
+    float* out = col < W ? dw : db;
+    if (out) out[col < W ? col : col - W] = (float)s;
+  }
+}
+
+// The widest row that teams hold in registers; wider ones take the loops over memory above.
+constexpr int64_t kMaxTeamWidth = 8192;
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// 16-byte loads and stores need every row of every operand to start on 16 bytes.
+template <typename T>
+bool vectors_fit(const Norm& n, const void* const* rows_of, const int64_t* ld, int count) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (n.W % VEC) return false;
+  for (int i = 0; i < count; ++i)
+    if (!aligned16(rows_of[i]) || ld[i] % VEC) return false;
+  return aligned16(n.gamma) && aligned16(n.beta) && aligned16(n.p) && aligned16(n.q);
+}
+
+// Calls f with the Shape for rows of W values: the smallest team that holds a row, 16 values a thread at most.
+template <typename T, typename F>
+int by_shape(int64_t W, bool vec, F f) {
+  constexpr int VEC = 16 / sizeof(T), V4 = 16 / VEC;
+  if (vec) {
+    if (W <= 4 * VEC) return f(Shape<T, VEC, 1, 4, V4>{});
+    if (W <= 8 * VEC) return f(Shape<T, VEC, 1, 8, V4>{});
+    if (W <= 16 * VEC) return f(Shape<T, VEC, 1, 16, V4>{});
+    if (W <= 32 * VEC) return f(Shape<T, VEC, 1, 32, V4>{});
+    if (VEC == 4 && W <= 256) return f(Shape<T, VEC, 2, 32, V4 / 2>{});
+    if (W <= 512) return f(Shape<T, VEC, V4, 32, 1>{});
+    if (W <= 1024) return f(Shape<T, VEC, V4, 64, 1>{});
+    if (W <= 2048) return f(Shape<T, VEC, V4, 128, 1>{});
+    if (W <= 4096) return f(Shape<T, VEC, V4, 256, 1>{});
+    return f(Shape<T, VEC, V4, 512, 1>{});
+  }
+  if (W <= 32) return f(Shape<T, 1, 4, 8, 2>{});
+  if (W <= 128) return f(Shape<T, 1, 4, 32, 2>{});
+  if (W <= 512) return f(Shape<T, 1, 16, 32, 1>{});
+  if (W <= 1024) return f(Shape<T, 1, 16, 64, 1>{});
+  if (W <= 2048) return f(Shape<T, 1, 16, 128, 1>{});
+  if (W <= 4096) return f(Shape<T, 1, 16, 256, 1>{});
+  return f(Shape<T, 1, 16, 512, 1>{});
+}
+
+// Partial rows of column sums, one per CTA of a row kernel.
+int64_t most_parts(int64_t rows, int64_t W) {
+  const int64_t most = W <= 1024 ? 148 * 16 : 148 * 8;
+  return rows < most ? rows : most;
+}
+
+// CTAs of a row kernel: as many as the device holds at once, never more than there are batches of rows.
+template <auto Kernel, class S>
+int row_grid(int64_t rows, int64_t W, int rb) {
+  static const int resident = [] {
+    int dev = 0, sms = 148, per = 1;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, Kernel, S::THREADS, 0);
+    return sms * (per > 0 ? per : 1);
+  }();
+  const int64_t batches = (rows + S::TEAMS * rb - 1) / (S::TEAMS * rb), most = most_parts(rows, W);
+  int64_t g = batches < resident ? batches : resident;
+  return (int)(g < most ? g : most);
+}
+
+int sum_parts(const float* part, int n_part, int64_t W, float* dw, float* db, cudaStream_t st) {
+  k_part_sum<<<(unsigned)((2 * W + 31) / 32), dim3(32, 32), 0, st>>>(part, n_part, (int)W, dw, db);
+  E2A_CHECK_LAUNCH();
+  return E2A_OK;
+}
+
 int grid_rows(int64_t rows) {
   int64_t b = (rows + kThreads / 32 - 1) / (kThreads / 32);
   return (int)(b > 148 * 64 ? 148 * 64 : b);
@@ -241,7 +765,10 @@ bool bad_shape(int64_t rows, int64_t W, int64_t ld) { return rows < 0 || W <= 0 
 
 bool bad_mode(int dtype, int act) { return dtype < 0 || dtype > 2 || (act != 0 && act != 1); }
 
-size_t part_bytes(int64_t rows, int64_t W) { return e2a_align_up((size_t)chunk_count(rows) * 2 * W * 8, 256); }
+size_t part_bytes(int64_t rows, int64_t W) {
+  return e2a_align_up(W <= kMaxTeamWidth ? (size_t)most_parts(rows, W) * 2 * W * 4 : (size_t)chunk_count(rows) * 2 * W * 8,
+                      256);
+}
 
 template <typename F>
 int by_type(int dtype, F f) {
@@ -271,6 +798,17 @@ int e2a_layer_norm_fwd(const void* x, int64_t ldx, int dtype, const float* gamma
   const Norm n{gamma, beta, nullptr, nullptr, W, act == 1};
   return by_type(dtype, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
+    if (W <= kMaxTeamWidth) {
+      const void* of[] = {x, y};
+      const int64_t ld[] = {ldx, W};
+      return by_shape<T>(W, vectors_fit<T>(n, of, ld, 2), [&](auto shape) -> int {
+        using S = decltype(shape);
+        const int grid = row_grid<&k_row_fwd<S>, S>(rows, W, S::RB);
+        k_row_fwd<S><<<grid, S::THREADS, 0, (cudaStream_t)stream>>>((const T*)x, ldx, n, rows, eps, (T*)y, mean, rstd);
+        E2A_CHECK_LAUNCH();
+        return E2A_OK;
+      });
+    }
     k_ln_fwd<T><<<grid_rows(rows), kThreads, 0, (cudaStream_t)stream>>>((const T*)x, ldx, n, rows, eps, (T*)y, mean,
                                                                         rstd);
     E2A_CHECK_LAUNCH();
@@ -293,6 +831,20 @@ int e2a_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy,
   const Norm n{gamma, beta, nullptr, nullptr, W, act == 1};
   return by_type(dtype, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
+    if (!dx && !dgamma && !dbeta) return E2A_OK;
+    if (W <= kMaxTeamWidth) {
+      const void* of[] = {x, dy, dx};
+      const int64_t ld[] = {ldx, lddy, W};
+      return by_shape<T>(W, vectors_fit<T>(n, of, ld, 3), [&](auto shape) -> int {
+        using S = decltype(shape);
+        float* part = dgamma || dbeta ? (float*)workspace : nullptr;
+        const int grid = row_grid<&k_row_bwd<S>, S>(rows, W, S::RB);
+        k_row_bwd<S><<<grid, S::THREADS, 0, st>>>((const T*)x, ldx, (const T*)dy, lddy, n, mean, rstd, rows, (T*)dx,
+                                                  part);
+        E2A_CHECK_LAUNCH();
+        return part ? sum_parts(part, grid, W, dgamma, dbeta, st) : E2A_OK;
+      });
+    }
     if (dx) {
       k_ln_bwd<T><<<grid_rows(rows), kThreads, 0, st>>>((const T*)x, ldx, (const T*)dy, lddy, n, mean, rstd, rows,
                                                         (T*)dx);
@@ -324,6 +876,21 @@ int e2a_layer_norm_bwd2(const void* x, int64_t ldx, const void* dy, int64_t lddy
   const Norm n{gamma, beta, p, q, W, act == 1};
   return by_type(dtype, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
+    if (W <= kMaxTeamWidth) {
+      const void* of[] = {x, dy, u, d_dy, dx};
+      const int64_t ld[] = {ldx, lddy, ldu, W, W};
+      return by_shape<T>(W, vectors_fit<T>(n, of, ld, 5), [&](auto shape) -> int {
+        using S = decltype(shape);
+        float* sums = dgamma || dbeta ? (float*)part : nullptr;
+        auto* kernel = p || q ? k_row_bwd2<S, true> : k_row_bwd2<S, false>;
+        const int grid = p || q ? row_grid<&k_row_bwd2<S, true>, S>(rows, W, 1)
+                                : row_grid<&k_row_bwd2<S, false>, S>(rows, W, 1);
+        kernel<<<grid, S::THREADS, 0, st>>>((const T*)x, ldx, (const T*)dy, lddy, (const T*)u, ldu, n, mean, rstd, rows,
+                                            (T*)d_dy, (T*)dx, sums);
+        E2A_CHECK_LAUNCH();
+        return sums ? sum_parts(sums, grid, W, dgamma, dbeta, st) : E2A_OK;
+      });
+    }
     k_ln_bwd2<T><<<grid_rows(rows), kThreads, 0, st>>>((const T*)x, ldx, (const T*)dy, lddy, (const T*)u, ldu, n, mean,
                                                        rstd, rows, (T*)d_dy, (T*)dx, row_u, row_c);
     E2A_CHECK_LAUNCH();
