@@ -409,7 +409,7 @@ int e2a_layer_norm_bwd2(const void* x, int64_t ldx, const void* dy, int64_t lddy
 /* state_bits 8: one byte an element and, per 256 of them, one scale byte: x = y 2^(scale - 127) with   */
 /* y a small float, m: sign, 4 exponent, 3 fraction bits; sqrt(v): 4 exponent, 4 fraction bits; exponent */
 /* 15 stands for [1, 2), 0 for the subnormals; scale 255 for a block of NaN.  e2a_moments_unpack gives   */
-/* m and v of n elements as fp32.  Tensors that overlap a parameter are refused (E2A_ERR_ARG).          */
+/* m and v of n elements (whole blocks) as fp32.  Tensors that overlap a parameter are refused (E2A_ERR_ARG).          */
 /* ------------------------------------------------------------------------------------------ */
 size_t e2a_grad_norm_workspace_bytes(int64_t n_tensors);
 int e2a_sum_squares(const uint64_t* tensors, const int64_t* numel, int64_t n_tensors, int dtype, void* workspace,

@@ -335,7 +335,7 @@ def test_parameters_without_gradient_and_groups():
     ps[1].grad = None
     opt.step()
     assert torch.equal(ps[1], start[1]) and not torch.equal(ps[0], start[0])
-    assert float((ps[2] - start[2]).abs().min()) > 0.3           # the second group's lr: the first step is lr sign(g)
+    assert float((ps[2].detach() - start[2]).abs().min()) > 0.3           # the second group's lr: the first step is lr sign(g)
     ps[1].grad = torch.ones_like(ps[1])
     opt.step()
     assert [int(opt.state[p]["step"]) for p in ps] == [2, 1, 2, 2, 2]

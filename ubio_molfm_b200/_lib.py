@@ -170,7 +170,12 @@ def ptr(t):
 
 
 def stream_of(device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    """The current stream of ``device`` (None: of the current device).  The raw handle: building a
+    ``torch.cuda.Stream`` around it costs as much as a launch."""
+    index = getattr(device, "index", device)
+    if not isinstance(index, int):
+        index = torch.cuda.current_device()
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))
 
 
 def require_cuda(*tensors):

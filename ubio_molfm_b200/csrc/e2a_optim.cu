@@ -29,15 +29,18 @@
 namespace {
 
 constexpr int kBlock = 256;          // elements that share a scale
+constexpr int kThreads = 256;
+constexpr int kUnit = 8 * kBlock;    // elements that a CTA takes at a time: one block a warp
 constexpr int kTensors = 512;        // tensors in one launch's table (18.4 KB of kernel parameters)
-constexpr int kNormCtas = 592;       // partial sums of squares of one launch (4 per SM)
+constexpr int kNormCtas = 1184;      // partial sums of squares of one launch (8 per SM)
+constexpr int kStepCtas = 148 * 16;  // CTAs of one step: contiguous ranges, a few waves so that they even out
 
 struct Table {
   uint64_t p[kTensors];
   uint64_t g[kTensors];
   int64_t numel[kTensors];
   int64_t offset[kTensors];
-  int32_t first[kTensors + 1];       // first block of every tensor
+  int32_t first[kTensors + 1];       // first unit of every tensor
   int32_t n;
 };
 
@@ -55,7 +58,7 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
-// The tensor that owns block b: the last j with first[j] <= b (empty tensors own none).
+// The tensor that owns unit b: the last j with first[j] <= b (empty tensors own none).
 __device__ __forceinline__ int tensor_of(const Table& t, int32_t b) {
   int lo = 0, hi = t.n;
   while (hi - lo > 1) {
@@ -159,139 +162,234 @@ __device__ __forceinline__ Moments update(float p, float g, float m, float v, co
   return o;
 }
 
+// Four neighbouring values of a tensor of n from element i on, 0 beyond its end; one load where the tensor's
+// address allows it (`vec`) and all four exist.
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p, int64_t i, int64_t n, bool vec) {
+  if (vec && i + 4 <= n) {
+    if (sizeof(T) == 4) return *reinterpret_cast<const float4*>(p + i);
+    const uint2 w = *reinterpret_cast<const uint2*>(p + i);
+    const T* h = reinterpret_cast<const T*>(&w);
+    return make_float4(to_f(h[0]), to_f(h[1]), to_f(h[2]), to_f(h[3]));
+  }
+  float4 v = f4_zero();
+  if (i < n) v.x = to_f(p[i]);
+  if (i + 1 < n) v.y = to_f(p[i + 1]);
+  if (i + 2 < n) v.z = to_f(p[i + 2]);
+  if (i + 3 < n) v.w = to_f(p[i + 3]);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, float4 v) {
+  const T h[4] = {from_f<T>(v.x), from_f<T>(v.y), from_f<T>(v.z), from_f<T>(v.w)};
+  if (vec && i + 4 <= n) {
+    if (sizeof(T) == 4)
+      *reinterpret_cast<float4*>(p + i) = v;
+    else
+      *reinterpret_cast<uint2*>(p + i) = *reinterpret_cast<const uint2*>(h);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k < n) p[i + k] = h[k];
+  }
+}
+
+// A CTA walks a contiguous range of units, 8 values a thread and unit: a warp owns one block of 256, lane l the
+// values 4 l and 128 + 4 l on (16-byte loads of fp32, 4-byte ones of codes, all neighbouring).
 template <typename T, int BITS>
-__global__ void __launch_bounds__(kBlock)
-k_adamw(const __grid_constant__ Table tab, int32_t n_blocks, void* __restrict__ exp_avg, void* __restrict__ exp_avg_sq,
-        uint8_t* __restrict__ scale_m, uint8_t* __restrict__ scale_v, const Scalars* __restrict__ scal,
-        const Globals* __restrict__ glob, float b1, float a1, float b2, float a2, float eps, bool clip) {
-  __shared__ uint32_t top[2][kBlock / 32];
+__global__ void __launch_bounds__(kThreads)
+k_adamw(const __grid_constant__ Table tab, int32_t n_units, int32_t per_cta, void* __restrict__ exp_avg,
+        void* __restrict__ exp_avg_sq, uint8_t* __restrict__ scale_m, uint8_t* __restrict__ scale_v,
+        const Scalars* __restrict__ scal, const Globals* __restrict__ glob, float b1, float a1, float b2, float a2,
+        float eps, bool clip) {
   const Globals gl = *glob;
   if (gl.skip) return;
-  for (int32_t b = blockIdx.x; b < n_blocks; b += gridDim.x) {
-    const int j = tensor_of(tab, b);
-    const int64_t i = (int64_t)(b - tab.first[j]) * kBlock + threadIdx.x;
-    const int64_t at = tab.offset[j] + i;
-    const bool in = i < tab.numel[j];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int32_t from = blockIdx.x * per_cta, to = min(from + per_cta, n_units);
+  int j = tensor_of(tab, from);
+  for (int32_t b = from; b < to; ++b) {
+    while (b >= tab.first[j + 1]) ++j;
+    const int64_t i0 = (int64_t)(b - tab.first[j]) * kUnit + warp * kBlock, n = tab.numel[j];
+    if (i0 >= n) continue;
+    const int64_t at = tab.offset[j] + i0;
     const Scalars s = scal[j];
     T* p = reinterpret_cast<T*>(tab.p[j]);
     const T* g = reinterpret_cast<const T*>(tab.g[j]);
+    const bool vec = ((tab.p[j] | tab.g[j]) & (4 * sizeof(T) - 1)) == 0;
+    float4 pv[2], gv[2], mv[2], vv[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int c = 4 * lane + 128 * k;
+      pv[k] = load4(p, i0 + c, n, vec);
+      gv[k] = load4(g, i0 + c, n, vec);
+    }
+    uint32_t cm[2], cv[2];
+    float sm = 0.f, ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int c = 4 * lane + 128 * k;
+      if (BITS == 32) {
+        mv[k] = *reinterpret_cast<const float4*>((const float*)exp_avg + at + c);
+        vv[k] = *reinterpret_cast<const float4*>((const float*)exp_avg_sq + at + c);
+      } else {
+        cm[k] = *reinterpret_cast<const uint32_t*>((const uint8_t*)exp_avg + at + c);
+        cv[k] = *reinterpret_cast<const uint32_t*>((const uint8_t*)exp_avg_sq + at + c);
+      }
+    }
+    if (BITS == 8) {
+      sm = scale_of(scale_m[at / kBlock]);
+      ss = scale_of(scale_v[at / kBlock]);
+    }
+    uint32_t top_m = 0, top_s = 0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float* pe = reinterpret_cast<float*>(&pv[k]);
+      float* me = reinterpret_cast<float*>(&mv[k]);
+      float* ve = reinterpret_cast<float*>(&vv[k]);
+      const float* ge = reinterpret_cast<const float*>(&gv[k]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (BITS == 8) {
+          me[e] = unpack_m((cm[k] >> (8 * e)) & 255u, sm);
+          const float r = unpack_s((cv[k] >> (8 * e)) & 255u, ss);
+          ve[e] = __fmul_rn(r, r);
+        }
+        const Moments o = update(pe[e], ge[e], me[e], ve[e], gl, s, b1, a1, b2, a2, eps, clip);
+        pe[e] = o.p;
+        me[e] = o.m;
+        ve[e] = o.v;
+        if (BITS == 8) {
+          if (i0 + 4 * lane + 128 * k + e >= n) me[e] = ve[e] = 0.f;   // a NaN block holds no more than its tensor
+          ve[e] = __fsqrt_rn(ve[e]);
+          top_m = max(top_m, __float_as_uint(me[e]) & 0x7FFFFFFFu);
+          top_s = max(top_s, __float_as_uint(ve[e]) & 0x7FFFFFFFu);
+        }
+      }
+      store4(p, i0 + 4 * lane + 128 * k, n, vec, pv[k]);
+    }
     if (BITS == 32) {
-      if (!in) continue;
-      float* m = (float*)exp_avg;
-      float* v = (float*)exp_avg_sq;
-      const Moments o = update(to_f(p[i]), to_f(g[i]), m[at], v[at], gl, s, b1, a1, b2, a2, eps, clip);
-      p[i] = from_f<T>(o.p);
-      m[at] = o.m;
-      v[at] = o.v;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int c = 4 * lane + 128 * k;
+        *reinterpret_cast<float4*>((float*)exp_avg + at + c) = mv[k];
+        *reinterpret_cast<float4*>((float*)exp_avg_sq + at + c) = vv[k];
+      }
     } else {
-      uint8_t* m = (uint8_t*)exp_avg;
-      uint8_t* v = (uint8_t*)exp_avg_sq;
-      Moments o{0.f, 0.f, 0.f};
-      float sv = 0.f;
-      if (in) {
-        const float r = unpack_s(v[at], scale_of(scale_v[at / kBlock]));
-        o = update(to_f(p[i]), to_f(g[i]), unpack_m(m[at], scale_of(scale_m[at / kBlock])), __fmul_rn(r, r), gl, s, b1,
-                   a1, b2, a2, eps, clip);
-        p[i] = from_f<T>(o.p);
-        sv = __fsqrt_rn(o.v);
+      const uint32_t em = shared_exponent(__reduce_max_sync(0xffffffffu, top_m), 3);
+      const uint32_t es = shared_exponent(__reduce_max_sync(0xffffffffu, top_s), 4);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int c = 4 * lane + 128 * k;
+        const float* me = reinterpret_cast<const float*>(&mv[k]);
+        const float* ve = reinterpret_cast<const float*>(&vv[k]);
+        uint32_t wm = 0, ws = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t u = mixed((uint32_t)(i0 + c + e), (uint32_t)s.t);
+          wm |= pack_m(me[e], em, u >> 12) << (8 * e);
+          ws |= pack_s(ve[e], es, u & 0x7FFFFu) << (8 * e);
+        }
+        *reinterpret_cast<uint32_t*>((uint8_t*)exp_avg + at + c) = wm;
+        *reinterpret_cast<uint32_t*>((uint8_t*)exp_avg_sq + at + c) = ws;
       }
-      const uint32_t lm = __reduce_max_sync(0xffffffffu, __float_as_uint(o.m) & 0x7FFFFFFFu);
-      const uint32_t lv = __reduce_max_sync(0xffffffffu, __float_as_uint(sv) & 0x7FFFFFFFu);
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) {
-        top[0][threadIdx.x >> 5] = lm;
-        top[1][threadIdx.x >> 5] = lv;
-      }
-      __syncthreads();
-      uint32_t em = 0, ev = 0;
-      for (int w = 0; w < kBlock / 32; ++w) {
-        em = max(em, top[0][w]);
-        ev = max(ev, top[1][w]);
-      }
-      em = shared_exponent(em, 3);
-      ev = shared_exponent(ev, 4);
-      if (in) {
-        const uint32_t u = mixed((uint32_t)i, (uint32_t)s.t);
-        m[at] = (uint8_t)pack_m(o.m, em, u >> 12);
-        v[at] = (uint8_t)pack_s(sv, ev, u & 0x7FFFFu);
-      }
-      if (threadIdx.x == 0) {
+      if (lane == 0) {
         scale_m[at / kBlock] = (uint8_t)em;
-        scale_v[at / kBlock] = (uint8_t)ev;
+        scale_v[at / kBlock] = (uint8_t)es;
       }
     }
   }
 }
 
-__global__ void k_moments_unpack(const uint8_t* __restrict__ m, const uint8_t* __restrict__ v,
-                                 const uint8_t* __restrict__ scale_m, const uint8_t* __restrict__ scale_v, int64_t n,
-                                 float* __restrict__ out_m, float* __restrict__ out_v) {
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-    out_m[i] = unpack_m(m[i], scale_of(scale_m[i / kBlock]));
-    const float s = unpack_s(v[i], scale_of(scale_v[i / kBlock]));
-    out_v[i] = __fmul_rn(s, s);
+// Whole blocks of 256, four values a thread at a time.
+__global__ void __launch_bounds__(kThreads)
+k_moments_unpack(const uint8_t* __restrict__ m, const uint8_t* __restrict__ v, const uint8_t* __restrict__ scale_m,
+                 const uint8_t* __restrict__ scale_v, int64_t n, float* __restrict__ out_m,
+                 float* __restrict__ out_v) {
+  for (int64_t i = 4 * (blockIdx.x * (int64_t)kThreads + threadIdx.x); i < n; i += 4 * (int64_t)gridDim.x * kThreads) {
+    const uint32_t cm = *reinterpret_cast<const uint32_t*>(m + i), cv = *reinterpret_cast<const uint32_t*>(v + i);
+    const float sm = scale_of(scale_m[i / kBlock]), ss = scale_of(scale_v[i / kBlock]);
+    float a[4], b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a[e] = unpack_m((cm >> (8 * e)) & 255u, sm);
+      const float r = unpack_s((cv >> (8 * e)) & 255u, ss);
+      b[e] = __fmul_rn(r, r);
+    }
+    *reinterpret_cast<float4*>(out_m + i) = make_float4(a[0], a[1], a[2], a[3]);
+    *reinterpret_cast<float4*>(out_v + i) = make_float4(b[0], b[1], b[2], b[3]);
   }
 }
 
 // ---- the global norm -------------------------------------------------------------------------------
-// Squares are exact in 64 bits and summed there: the norm is the correctly rounded one but for ties.
-template <typename T>
-__global__ void __launch_bounds__(kBlock)
-k_sum_squares(const __grid_constant__ Table tab, int32_t n_blocks, double* __restrict__ part) {
-  __shared__ double sh[kBlock / 32];
-  double s = 0.;
-  for (int32_t b = blockIdx.x; b < n_blocks; b += gridDim.x) {
-    const int j = tensor_of(tab, b);
-    const int64_t i = (int64_t)(b - tab.first[j]) * kBlock + threadIdx.x;
-    if (i < tab.numel[j]) {
-      const double g = (double)to_f(reinterpret_cast<const T*>(tab.g[j])[i]);
-      s += g * g;
-    }
-  }
+__device__ __forceinline__ double cta_sum(double s, double* sh) {
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kBlock / 32; ++w) s += sh[w];
-    part[blockIdx.x] = s;
-  }
+  s = 0.;
+  for (int w = 0; w < kThreads / 32; ++w) s += sh[w];
+  return s;
 }
 
-__global__ void k_norm(const double* __restrict__ part, int64_t n, float* __restrict__ norm) {
-  __shared__ double sh[kBlock / 32];
-  double s = 0.;
-  for (int64_t i = threadIdx.x; i < n; i += kBlock) s += part[i];
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kBlock / 32; ++w) s += sh[w];
-    *norm = (float)sqrt(s);
+// Squares are exact in 64 bits and summed there: the norm is the correctly rounded one but for ties.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+k_sum_squares(const __grid_constant__ Table tab, int32_t n_units, int32_t per_cta, double* __restrict__ part) {
+  __shared__ double sh[kThreads / 32];
+  double s[2] = {0., 0.};
+  const int32_t from = blockIdx.x * per_cta, to = min(from + per_cta, n_units);
+  int j = tensor_of(tab, from);
+  for (int32_t b = from; b < to; ++b) {
+    while (b >= tab.first[j + 1]) ++j;
+    const int64_t i0 = (int64_t)(b - tab.first[j]) * kUnit, n = tab.numel[j];
+    const T* g = reinterpret_cast<const T*>(tab.g[j]);
+    const bool vec = (tab.g[j] & (4 * sizeof(T) - 1)) == 0;
+    float4 v[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) v[k] = load4(g, i0 + 4 * (threadIdx.x + kThreads * k), n, vec);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      s[0] = fma((double)v[k].x, (double)v[k].x, s[0]);
+      s[1] = fma((double)v[k].y, (double)v[k].y, s[1]);
+      s[0] = fma((double)v[k].z, (double)v[k].z, s[0]);
+      s[1] = fma((double)v[k].w, (double)v[k].w, s[1]);
+    }
   }
+  const double all = cta_sum(s[0] + s[1], sh);
+  if (threadIdx.x == 0) part[blockIdx.x] = all;
+}
+
+__global__ void __launch_bounds__(kThreads)
+k_norm(const double* __restrict__ part, int64_t n, float* __restrict__ norm) {
+  __shared__ double sh[kThreads / 32];
+  double s = 0.;
+  for (int64_t i = threadIdx.x; i < n; i += kThreads) s += part[i];
+  s = cta_sum(s, sh);
+  if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
 int64_t blocks_of(int64_t numel) { return (numel + kBlock - 1) / kBlock; }
+int64_t units_of(int64_t numel) { return (numel + kUnit - 1) / kUnit; }
 
 size_t width_of(int dtype) { return dtype == 0 ? 4 : 2; }
 
-// Fills a launch's table with tensors [from, ...): as many as fit.  Returns the next tensor, blocks in *n_blocks.
+// Fills a launch's table with tensors [from, ...): as many as fit.  Returns the next tensor, units in *n_units.
 int64_t fill(Table* t, int64_t from, int64_t n_tensors, const uint64_t* p, const uint64_t* g, const int64_t* numel,
-             const int64_t* offset, int32_t* n_blocks) {
-  int64_t blocks = 0, j = from;
+             const int64_t* offset, int32_t* n_units) {
+  int64_t units = 0, j = from;
   int k = 0;
   for (; j < n_tensors && k < kTensors; ++j, ++k) {
-    const int64_t nb = blocks_of(numel[j]);
-    if (k > 0 && blocks + nb > (1ll << 30)) break;
+    const int64_t nu = units_of(numel[j]);
+    if (k > 0 && units + nu > (1ll << 30)) break;
     t->p[k] = p ? p[j] : 0;
     t->g[k] = g[j];
     t->numel[k] = numel[j];
     t->offset[k] = offset ? offset[j] : 0;
-    t->first[k] = (int32_t)blocks;
-    blocks += nb;
+    t->first[k] = (int32_t)units;
+    units += nu;
   }
-  t->first[k] = (int32_t)blocks;
+  t->first[k] = (int32_t)units;
   t->n = k;
-  *n_blocks = (int32_t)blocks;
+  *n_units = (int32_t)units;
   return j;
 }
 
@@ -308,13 +406,17 @@ struct Span { uint64_t begin, end; bool written; };
 int overlap(const uint64_t* p, const uint64_t* g, const int64_t* numel, int64_t n, size_t width, bool* found) {
   Span* s = new (std::nothrow) Span[2 * n + 1];
   if (!s) return E2A_ERR_WORKSPACE;
-  int64_t k = 0;
-  for (int64_t j = 0; j < n; ++j) {
-    if (numel[j] == 0) continue;
-    s[k++] = {p[j], p[j] + (uint64_t)numel[j] * width, true};
-    s[k++] = {g[j], g[j] + (uint64_t)numel[j] * width, false};
-  }
-  std::sort(s, s + k, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  const auto before = [](const Span& a, const Span& b) { return a.begin < b.begin; };
+  int64_t k = 0, half = 0;
+  for (int64_t j = 0; j < n; ++j)
+    if (numel[j] > 0) s[k++] = {p[j], p[j] + (uint64_t)numel[j] * width, true};
+  half = k;
+  for (int64_t j = 0; j < n; ++j)
+    if (numel[j] > 0) s[k++] = {g[j], g[j] + (uint64_t)numel[j] * width, false};
+  // lists in the order of their addresses, as one allocation's views are, need no sort
+  if (!std::is_sorted(s, s + half, before)) std::sort(s, s + half, before);
+  if (!std::is_sorted(s + half, s + k, before)) std::sort(s + half, s + k, before);
+  if (half < k && half > 0 && before(s[half], s[half - 1])) std::sort(s, s + k, before);
   uint64_t written = 0, any = 0;      // furthest ends so far
   *found = false;
   for (int64_t i = 0; i < k; ++i) {
@@ -333,8 +435,6 @@ int by_type(int dtype, F f) {
   return f((__half*)nullptr);
 }
 
-int grid_of(int32_t n_blocks) { return n_blocks < 148 * 8 ? n_blocks : 148 * 8; }
-
 }  // namespace
 
 extern "C" {
@@ -351,14 +451,14 @@ int e2a_sum_squares(const uint64_t* tensors, const int64_t* numel, int64_t n_ten
   const int64_t room = (int64_t)(workspace_bytes / sizeof(double));
   for (int64_t j = 0; j < n_tensors;) {
     static thread_local Table t;
-    int32_t blocks = 0;
-    j = fill(&t, j, n_tensors, nullptr, tensors, numel, nullptr, &blocks);
-    if (blocks == 0) continue;
-    const int ctas = blocks < kNormCtas ? blocks : kNormCtas;
+    int32_t units = 0;
+    j = fill(&t, j, n_tensors, nullptr, tensors, numel, nullptr, &units);
+    if (units == 0) continue;
+    const int32_t per = (units + kNormCtas - 1) / kNormCtas, ctas = (units + per - 1) / per;
     if (!part || *n_partials + ctas > room) return E2A_ERR_WORKSPACE;
     const int rc = by_type(dtype, [&](auto* x) -> int {
       using T = std::remove_pointer_t<decltype(x)>;
-      k_sum_squares<T><<<ctas, kBlock, 0, (cudaStream_t)stream>>>(t, blocks, part + *n_partials);
+      k_sum_squares<T><<<ctas, kThreads, 0, (cudaStream_t)stream>>>(t, units, per, part + *n_partials);
       E2A_CHECK_LAUNCH();
       return E2A_OK;
     });
@@ -370,7 +470,7 @@ int e2a_sum_squares(const uint64_t* tensors, const int64_t* numel, int64_t n_ten
 
 int e2a_norm_of_squares(const void* partials, int64_t n_partials, float* norm, void* stream) {
   if (n_partials < 0 || (n_partials > 0 && !partials) || !norm) return E2A_ERR_ARG;
-  k_norm<<<1, kBlock, 0, (cudaStream_t)stream>>>((const double*)partials, n_partials, norm);
+  k_norm<<<1, kThreads, 0, (cudaStream_t)stream>>>((const double*)partials, n_partials, norm);
   E2A_CHECK_LAUNCH();
   return E2A_OK;
 }
@@ -412,17 +512,18 @@ int e2a_adamw_step(const uint64_t* params, const uint64_t* grads, const int64_t*
     static thread_local Table t;
     static thread_local Slots slot;
     const int64_t from = j;
-    int32_t blocks = 0;
-    j = fill(&t, j, n_tensors, params, grads, numel, state_offset, &blocks);
+    int32_t units = 0;
+    j = fill(&t, j, n_tensors, params, grads, numel, state_offset, &units);
     std::copy(slots + from, slots + j, slot.slot);
     k_adamw_scalars<<<1, kTensors, 0, st>>>(slot, h, step, t.n, scal + from, glob);
     E2A_CHECK_LAUNCH();
-    if (blocks == 0) continue;
+    if (units == 0) continue;
     rc = by_type(dtype, [&](auto* x) -> int {
       using T = std::remove_pointer_t<decltype(x)>;
       auto* kernel = state_bits == 32 ? k_adamw<T, 32> : k_adamw<T, 8>;
-      kernel<<<grid_of(blocks), kBlock, 0, st>>>(t, blocks, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale,
-                                                 scal + from, glob, b1, a1, b2, a2, (float)eps, grad_norm != nullptr);
+      const int32_t per = (units + kStepCtas - 1) / kStepCtas, ctas = (units + per - 1) / per;
+      kernel<<<ctas, kThreads, 0, st>>>(t, units, per, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale,
+                                        scal + from, glob, b1, a1, b2, a2, (float)eps, grad_norm != nullptr);
       E2A_CHECK_LAUNCH();
       return E2A_OK;
     });
@@ -436,8 +537,9 @@ int e2a_moments_unpack(const uint8_t* exp_avg, const uint8_t* exp_avg_sq, const 
   if (n < 0) return E2A_ERR_ARG;
   if (n == 0) return E2A_OK;
   if (!exp_avg || !exp_avg_sq || !exp_avg_scale || !exp_avg_sq_scale || !out_avg || !out_avg_sq) return E2A_ERR_ARG;
-  const int64_t b = blocks_of(n);
-  k_moments_unpack<<<(int)(b < 148 * 32 ? b : 148 * 32), kBlock, 0, (cudaStream_t)stream>>>(
+  if (n % kBlock) return E2A_ERR_ARG;
+  const int64_t b = n / (4 * kThreads) + 1;
+  k_moments_unpack<<<(int)(b < 148 * 16 ? b : 148 * 16), kThreads, 0, (cudaStream_t)stream>>>(
       exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, n, out_avg, out_avg_sq);
   E2A_CHECK_LAUNCH();
   return E2A_OK;

@@ -10,14 +10,10 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import check, ptr, require_cuda, stream_of
+from ._lib import check, require_cuda, stream_of
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {None: 0, "silu": 1}
-
-
-def _workspace(nbytes, device):
-    return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
 
 
 def _rows(t, width):
@@ -31,42 +27,63 @@ def _rows(t, width):
 
 
 def _f32(t):
-    return None if t is None else t.contiguous().to(torch.float32)
+    """A contiguous fp32 vector (itself where it is one) and its address; None stays None."""
+    if t is None:
+        return None, None
+    if t.dtype != torch.float32 or not t.is_contiguous():
+        t = t.contiguous().to(torch.float32)
+    return t, t.data_ptr()
 
 
-def _backward(x, g, weight, bias, mean, rstd, act, need_x, need_cols):
+def _columns(lib_bytes, rows, width, dev):
+    """Storage of a column-sum pass: (dw, db) [width] fp32 and the workspace."""
+    dw, db = torch.empty((2, width), dtype=torch.float32, device=dev).unbind(0)
+    ws = torch.empty(max(lib_bytes(rows, width), 1), dtype=torch.uint8, device=dev)
+    return dw, db, ws
+
+
+def _backward(x, g, weight, bias, stats, act, need_x, need_cols):
     """``(dx, dw, db)`` of rows: dx in x's dtype (or None), dw / db [width] in fp32 (or None)."""
     lib = _lib.load()
-    width = x.shape[-1]
+    width, dev = x.shape[-1], x.device
     x2, ldx = _rows(x, width)
     g2, ldg = _rows(g, width)
-    rows, dev = x2.shape[0], x.device
+    rows = x2.shape[0]
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-    cols = torch.empty((2, width), dtype=torch.float32, device=dev) if need_cols else None
-    ws = _workspace(lib.e2a_layer_norm_bwd_workspace_bytes(rows, width) if need_cols else 0, dev)
-    check(lib.e2a_layer_norm_bwd(ptr(x2), ldx, ptr(g2), ldg, _DTYPES[x.dtype], ptr(weight), ptr(bias), ptr(mean),
-                                 ptr(rstd), rows, width, act, ptr(dx), None if cols is None else ptr(cols[0]),
-                                 None if cols is None else ptr(cols[1]), ptr(ws), ws.numel(), stream_of(dev)),
-          "e2a_layer_norm_bwd")
-    return dx, (None if cols is None else cols[0]), (None if cols is None else cols[1])
+    dw = db = ws = None
+    if need_cols:
+        dw, db, ws = _columns(lib.e2a_layer_norm_bwd_workspace_bytes, rows, width, dev)
+    w, w_at = _f32(weight)
+    b, b_at = _f32(bias)
+    at = stats.data_ptr()
+    check(lib.e2a_layer_norm_bwd(x2.data_ptr(), ldx, g2.data_ptr(), ldg, _DTYPES[x.dtype], w_at, b_at, at,
+                                 at + 4 * rows, rows, width, act, dx.data_ptr() if need_x else None,
+                                 dw.data_ptr() if need_cols else None, db.data_ptr() if need_cols else None,
+                                 ws.data_ptr() if need_cols else None, ws.numel() if need_cols else 0,
+                                 stream_of(dev)), "e2a_layer_norm_bwd")
+    return dx, dw, db
 
 
 def _cast(t, like):
-    return None if t is None or like is None else t.to(like.dtype)
+    if t is None or like is None:
+        return None
+    return t if like.dtype == torch.float32 else t.to(like.dtype)
 
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, act):
         lib = _lib.load()
-        width = x.shape[-1]
+        width, dev = x.shape[-1], x.device
         x2, ldx = _rows(x, width)
-        rows, dev = x2.shape[0], x.device
+        rows = x2.shape[0]
         y = torch.empty(x.shape, dtype=x.dtype, device=dev)
         stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
-        w, b = _f32(weight), _f32(bias)
-        check(lib.e2a_layer_norm_fwd(ptr(x2), ldx, _DTYPES[x.dtype], ptr(w), ptr(b), rows, width, eps, act, ptr(y),
-                                     ptr(stats[0]), ptr(stats[1]), stream_of(dev)), "e2a_layer_norm_fwd")
+        w, w_at = _f32(weight)
+        b, b_at = _f32(bias)
+        at = stats.data_ptr()
+        check(lib.e2a_layer_norm_fwd(x2.data_ptr(), ldx, _DTYPES[x.dtype], w_at, b_at, rows, width, eps, act,
+                                     y.data_ptr(), at, at + 4 * rows, stream_of(dev)), "e2a_layer_norm_fwd")
         ctx.save_for_backward(x, weight, bias, stats)
         ctx.act = act
         return y
@@ -79,7 +96,7 @@ class _LayerNormFn(torch.autograd.Function):
             dx, dw, db = _LayerNormBackwardFn.apply(g, x, weight, bias, stats, ctx.act)
             return dx, dw, db, None, None
         need = ctx.needs_input_grad
-        dx, dw, db = _backward(x, g, _f32(weight), _f32(bias), stats[0], stats[1], ctx.act, need[0], need[1] or need[2])
+        dx, dw, db = _backward(x, g, weight, bias, stats, ctx.act, need[0], need[1] or need[2])
         return dx, _cast(dw, weight) if need[1] else None, _cast(db, bias) if need[2] else None, None, None
 
 
@@ -89,8 +106,7 @@ class _LayerNormBackwardFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, g, x, weight, bias, stats, act):
         ctx.set_materialize_grads(False)
-        dx, dw, db = _backward(x, g, _f32(weight), _f32(bias), stats[0], stats[1], act, True,
-                               weight is not None or bias is not None)
+        dx, dw, db = _backward(x, g, weight, bias, stats, act, True, weight is not None or bias is not None)
         ctx.save_for_backward(g, x, weight, bias, stats)
         ctx.act = act
         return dx, _cast(dw, weight), _cast(db, bias)
@@ -103,32 +119,30 @@ class _LayerNormBackwardFn(torch.autograd.Function):
         if u is None and p is None and q is None:
             return None, None, None, None, None, None
         lib = _lib.load()
-        width = x.shape[-1]
+        width, dev = x.shape[-1], x.device
         if u is None:
-            u = torch.zeros((), dtype=x.dtype, device=x.device).expand(x.shape)
+            u = torch.zeros((), dtype=x.dtype, device=dev).expand(x.shape)
         x2, ldx = _rows(x, width)
         g2, ldg = _rows(g, width)
         u2, ldu = _rows(u, width)
-        rows, dev = x2.shape[0], x.device
-        w, b, p, q = _f32(weight), _f32(bias), _f32(p), _f32(q)
+        rows = x2.shape[0]
+        (w, w_at), (b, b_at), (p, p_at), (q, q_at) = _f32(weight), _f32(bias), _f32(p), _f32(q)
         d_g = torch.empty(x.shape, dtype=x.dtype, device=dev)
         d_x = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        need_cols = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
-        cols = torch.empty((2, width), dtype=torch.float32, device=dev) if need_cols else None
-        ws = _workspace(lib.e2a_layer_norm_bwd2_workspace_bytes(rows, width), dev)
-        check(lib.e2a_layer_norm_bwd2(ptr(x2), ldx, ptr(g2), ldg, ptr(u2), ldu, _DTYPES[x.dtype], ptr(w), ptr(b),
-                                      ptr(stats[0]), ptr(stats[1]), ptr(p), ptr(q), rows, width, ctx.act, ptr(d_g),
-                                      ptr(d_x), None if cols is None else ptr(cols[0]),
-                                      None if cols is None else ptr(cols[1]), ptr(ws), ws.numel(), stream_of(dev)),
-              "e2a_layer_norm_bwd2")
-        return (d_g, d_x, None if weight is None or cols is None else _cast(cols[0], weight),
-                None if bias is None or cols is None else _cast(cols[1], bias), None, None)
+        dw, db, ws = _columns(lib.e2a_layer_norm_bwd2_workspace_bytes, rows, width, dev)
+        cols = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
+        at = stats.data_ptr()
+        check(lib.e2a_layer_norm_bwd2(x2.data_ptr(), ldx, g2.data_ptr(), ldg, u2.data_ptr(), ldu, _DTYPES[x.dtype],
+                                      w_at, b_at, at, at + 4 * rows, p_at, q_at, rows, width, ctx.act, d_g.data_ptr(),
+                                      d_x.data_ptr(), dw.data_ptr() if cols else None, db.data_ptr() if cols else None,
+                                      ws.data_ptr(), ws.numel(), stream_of(dev)), "e2a_layer_norm_bwd2")
+        return d_g, d_x, _cast(dw, weight) if cols else None, _cast(db, bias) if cols else None, None, None
 
 
 def _check_affine(name, t, x):
     if t is None:
         return
-    if t.shape != x.shape[-1:]:
+    if t.dim() != 1 or t.shape[0] != x.shape[-1]:
         raise ValueError(f"{name} must be [{x.shape[-1]}], got {list(t.shape)}")
     if t.dtype not in (torch.float32, x.dtype):
         raise TypeError(f"{name} must be float32 or {x.dtype}, got {t.dtype}")
@@ -152,5 +166,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, activation=None):
         raise ValueError(f"activation={activation!r}: expected None or 'silu'")
     _check_affine("weight", weight, x)
     _check_affine("bias", bias, x)
+    if x.device.index == torch.cuda.current_device():
+        return _LayerNormFn.apply(x, weight, bias, float(eps), _ACTIVATIONS[activation])
     with torch.cuda.device(x.device):
         return _LayerNormFn.apply(x, weight, bias, float(eps), _ACTIVATIONS[activation])

@@ -8,6 +8,7 @@ pipeline/trainer.py:397-414), so a training step can be captured in a CUDA graph
 from __future__ import annotations
 
 from array import array
+from operator import attrgetter
 
 import torch
 
@@ -16,6 +17,9 @@ from ._lib import check, ptr, require_cuda, stream_of
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 BLOCK = 256          # elements that share a scale; every tensor's state starts at a multiple
+
+
+_dtype = attrgetter("dtype")
 
 
 def _address(a):
@@ -34,29 +38,51 @@ def _one_device(tensors, what):
     return tensors[0].device
 
 
+def _contiguous(tensors):
+    """``tensors``, with contiguous copies in the place of those that are not."""
+    try:
+        if all(map(torch.Tensor.is_contiguous, tensors)):
+            return tensors
+    except RuntimeError:
+        pass                 # a sparse tensor has no such notion
+    if any(t.layout != torch.strided for t in tensors):
+        raise TypeError("expected strided tensors")
+    return [t.contiguous() for t in tensors]
+
+
+def _by_type(what, tensors, *others):
+    """``[(dtype, tensors, *others)]``: the lists split by the tensors' types."""
+    kinds = set(map(_dtype, tensors))
+    if not kinds <= _DTYPES.keys():
+        raise TypeError(f"{what} takes float32, bfloat16 or float16 tensors, got {kinds - _DTYPES.keys()}")
+    if len(kinds) == 1:
+        return [(*kinds, tensors, *others)]
+    keep = {d: [k for k, t in enumerate(tensors) if t.dtype == d] for d in _DTYPES if d in kinds}
+    return [(d, *([x[k] for k in ks] for x in (tensors, *others))) for d, ks in keep.items()]
+
+
+@torch.no_grad()
 def grad_norm(tensors):
     """The global L2 norm ``sqrt(sum of all squares)`` of ``tensors`` (float32, bfloat16 or float16 on one CUDA
     device, any shapes) as a 0-dim float32 tensor there: sums in 64 bits, in a fixed order, no host read.  An
     empty list has norm 0 on the current device."""
-    tensors = list(tensors)
+    tensors = _contiguous(list(tensors))
     dev = _one_device(tensors, "the tensors") if tensors else torch.device("cuda", torch.cuda.current_device())
-    lib = _lib.load()
-    by_type = {}
-    for t in tensors:
-        if t.layout != torch.strided or t.dtype not in _DTYPES:
-            raise TypeError(f"grad_norm takes strided float32, bfloat16 or float16 tensors, got {t.dtype}, {t.layout}")
-        by_type.setdefault(t.dtype, []).append(t.detach().contiguous())
-    with torch.cuda.device(dev):
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        size = sum(lib.e2a_grad_norm_workspace_bytes(len(ts)) for ts in by_type.values())
-        ws = torch.empty(max(size, 8), dtype=torch.uint8, device=dev)
-        done, count = 0, array("q", [0])
-        for dtype, ts in by_type.items():
-            pt, num = _pointers(ts), array("q", map(torch.Tensor.numel, ts))
-            check(lib.e2a_sum_squares(_address(pt), _address(num), len(ts), _DTYPES[dtype], ws.data_ptr() + 8 * done,
-                                      ws.numel() - 8 * done, _address(count), stream_of(dev)), "e2a_sum_squares")
-            done += count[0]
-        check(lib.e2a_norm_of_squares(ptr(ws), done, ptr(norm), stream_of(dev)), "e2a_norm_of_squares")
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return grad_norm(tensors)
+    lib, stream = _lib.load(), stream_of(dev)
+    lists = _by_type("grad_norm", tensors) if tensors else []
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    size = sum(lib.e2a_grad_norm_workspace_bytes(len(ts)) for _, ts in lists)
+    ws = torch.empty(max(size, 8), dtype=torch.uint8, device=dev)
+    at, done, count = ws.data_ptr(), 0, array("q", [0])
+    for dtype, ts in lists:
+        pt, num = _pointers(ts), array("q", map(torch.Tensor.numel, ts))
+        check(lib.e2a_sum_squares(_address(pt), _address(num), len(ts), _DTYPES[dtype], at + 8 * done, size - 8 * done,
+                                  _address(count), stream), "e2a_sum_squares")
+        done += count[0]
+    check(lib.e2a_norm_of_squares(at, done, norm.data_ptr(), stream), "e2a_norm_of_squares")
     return norm
 
 
@@ -66,11 +92,11 @@ class _Flat:
 
     def __init__(self, params, bits):
         self.device = _one_device(params, "a group's parameters")
-        self.numel = [p.numel() for p in params]
-        self.offset, end = [], 0
+        self.numel, self.offset, end = array("q", map(torch.Tensor.numel, params)), array("q"), 0
         for n in self.numel:
             self.offset.append(end)
             end += -(-n // BLOCK) * BLOCK
+        self.slot = array("i", range(len(params)))
         self.elements, self.bits = end, bits
         kind = torch.float32 if bits == 32 else torch.uint8
         self.buffers = {"step": torch.zeros(len(params), dtype=torch.int32, device=self.device),
@@ -212,69 +238,52 @@ class AdamW(torch.optim.Optimizer):
         work = []
         for gi, g in enumerate(self.param_groups):
             params = g["params"]
-            grads = [p.grad for p in params]
+            grads, index = [p.grad for p in params], None
             if any(t is None for t in grads):
                 index = [k for k, t in enumerate(grads) if t is not None]
                 params, grads = [params[k] for k in index], [grads[k] for k in index]
-            else:
-                index = None
             if grads:
-                work.append((gi, g, params, grads, index))
-        if not work:
-            return loss
+                work.append((gi, g, params, _contiguous(grads), index))
         norm = None
-        if self.max_grad_norm is not None:
+        if work and self.max_grad_norm is not None:
             norm = self.last_grad_norm = grad_norm([t for w in work for t in w[3]])
-        for gi, g, params, grads, index in work:
-            self._step_group(gi, g, params, grads, index, norm)
+        for w in work:
+            self._step_group(*w, norm)
         return loss
 
     def _step_group(self, gi, group, params, grads, index, norm):
         flat = self._group_state(gi)
         dev = flat.device
-        if index is None:
-            index = range(len(params))
         if _one_device(params, "a group's parameters") != dev:
             raise ValueError("the parameters have moved to another device than their state")
-        if norm is not None and norm.device != dev:
-            norm = norm.to(dev)
+        if dev.index != torch.cuda.current_device():
+            with torch.cuda.device(dev):
+                return self._step_group(gi, group, params, grads, index, norm)
         if not all(map(torch.Tensor.is_contiguous, params)):
             raise ValueError("AdamW takes contiguous parameters")
-        grads = [t if t.is_contiguous() else t.contiguous() for t in map(_dense, grads)]
-        if list(map(torch.Tensor.numel, params)) != [flat.numel[k] for k in index]:
+        numel, offset, slot = flat.numel, flat.offset, flat.slot
+        if index is not None:
+            numel, offset, slot = (array(a.typecode, [a[k] for k in index]) for a in (numel, offset, slot))
+        if array("q", map(torch.Tensor.numel, params)) != numel:
             raise ValueError("a parameter has changed its size since its state was made")
-        lr = group["lr"]
+        lr, lr_at = group["lr"], None
         if isinstance(lr, torch.Tensor) and lr.is_cuda:
             if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev:
                 raise ValueError("a tensor lr must be one float32 value on the parameters' device")
-        else:
-            lr = float(lr)
-        by_type = {}
-        for k, p, t in zip(index, params, grads):
-            by_type.setdefault(p.dtype, []).append((k, p, t))
-        lib, b = _lib.load(), flat.buffers
-        with torch.cuda.device(dev):
-            for dtype, items in by_type.items():
-                if dtype not in _DTYPES:
-                    raise TypeError(f"AdamW takes float32, bfloat16 or float16 parameters, got {dtype}")
-                pp, pg = _pointers([p for _, p, _ in items]), _pointers([t for _, _, t in items])
-                num = array("q", [flat.numel[k] for k, _, _ in items])
-                off = array("q", [flat.offset[k] for k, _, _ in items])
-                slot = array("i", [k for k, _, _ in items])
-                ws = torch.empty(lib.e2a_adamw_workspace_bytes(len(items)), dtype=torch.uint8, device=dev)
-                tensor_lr = isinstance(lr, torch.Tensor)
-                check(lib.e2a_adamw_step(
-                    _address(pp), _address(pg), _address(num), _address(off), _address(slot), len(items),
-                    _DTYPES[dtype], flat.bits, ptr(b["exp_avg"]), ptr(b["exp_avg_sq"]), ptr(b.get("exp_avg_scale")),
-                    ptr(b.get("exp_avg_sq_scale")), flat.elements, ptr(b["step"]), 0.0 if tensor_lr else lr,
-                    ptr(lr) if tensor_lr else None, float(group["betas"][0]), float(group["betas"][1]),
-                    float(group["eps"]), float(group["weight_decay"]), ptr(norm), float(self.max_grad_norm or 0.0),
-                    ptr(ws), ws.numel(), stream_of(dev)), "e2a_adamw_step")
+            lr, lr_at = 0.0, lr.data_ptr()
+        (beta1, beta2), b = group["betas"], flat.buffers
+        lib, stream = _lib.load(), stream_of(dev)
+        m, v, ms, vs, step = (b[k].data_ptr() if k in b else None for k in (
+            "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "step"))
+        for dtype, ps, gs, num, off, slots in _by_type("AdamW", params, grads, numel, offset, slot):
+            num, off, slots = (a if isinstance(a, array) else array(t, a)
+                               for t, a in (("q", num), ("q", off), ("i", slots)))
+            pp, pg = _pointers(ps), _pointers(gs)
+            ws = torch.empty(lib.e2a_adamw_workspace_bytes(len(ps)), dtype=torch.uint8, device=dev)
+            check(lib.e2a_adamw_step(
+                _address(pp), _address(pg), _address(num), _address(off), _address(slots), len(ps), _DTYPES[dtype],
+                flat.bits, m, v, ms, vs, flat.elements, step, lr, lr_at, beta1, beta2, group["eps"],
+                group["weight_decay"], None if norm is None else norm.data_ptr(), self.max_grad_norm or 0.0,
+                ws.data_ptr(), ws.numel(), stream), "e2a_adamw_step")
         # the kernels write behind autograd's back: saved tensors and caches keyed on versions have to see it
         torch.autograd.graph.increment_version(params)
-
-
-def _dense(t):
-    if t.layout != torch.strided:
-        raise TypeError("AdamW takes strided gradients")
-    return t
