@@ -99,6 +99,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_tensors = None
 
 
 E2A_ERR_UNSUPPORTED = 4   # status of an entry point that does not take the given operands (include/e2a.h)
@@ -123,6 +124,21 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def load_tensors():
+    """``libe2a_tensors.so``, which reads a list of tensors in one call (with the interpreter's lock held)."""
+    global _tensors
+    if _tensors is None:
+        path = os.path.join(_HERE, "libe2a_tensors.so")
+        if not os.path.exists(path):
+            raise E2AError(f"libe2a_tensors.so not found at {path}: build it with `python __graft_entry__.py` "
+                           "or `make -C ubio_molfm_b200/csrc`")
+        lib = ctypes.PyDLL(path)
+        lib.e2a_tensor_table.restype = I32
+        lib.e2a_tensor_table.argtypes = [ctypes.py_object, I64, P, P, P, P, P]
+        _tensors = lib
+    return _tensors
 
 
 def launch_count() -> int:

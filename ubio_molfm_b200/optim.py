@@ -30,6 +30,19 @@ def _pointers(tensors):
     return array("Q", map(torch.Tensor.data_ptr, tensors))
 
 
+def _table(tensors, with_grads=False):
+    """``(addresses, sizes, addresses of the gradients or None, type code, device index)`` of a list of tensors
+    in one call, or None where they are not all alike (see ``csrc/e2a_tensors.cpp``)."""
+    n = len(tensors)
+    at, numel, two = array("Q", (0,)) * n, array("q", (0,)) * n, array("i", (0, 0))
+    grads = array("Q", (0,)) * n if with_grads else None
+    if _lib.load_tensors().e2a_tensor_table(tensors, n, _address(at), _address(numel),
+                                            _address(grads) if with_grads else None, _address(two),
+                                            _address(two) + 4):
+        return None
+    return at, numel, grads, two[0], two[1]
+
+
 def _one_device(tensors, what):
     devices = set(map(torch.Tensor.get_device, tensors))
     if len(devices) > 1 or min(devices) < 0:
@@ -39,51 +52,53 @@ def _one_device(tensors, what):
 
 
 def _contiguous(tensors):
-    """``tensors``, with contiguous copies in the place of those that are not."""
-    try:
-        if all(map(torch.Tensor.is_contiguous, tensors)):
-            return tensors
-    except RuntimeError:
-        pass                 # a sparse tensor has no such notion
     if any(t.layout != torch.strided for t in tensors):
         raise TypeError("expected strided tensors")
-    return [t.contiguous() for t in tensors]
+    return [t.detach().contiguous() for t in tensors]
 
 
 def _by_type(what, tensors, *others):
-    """``[(dtype, tensors, *others)]``: the lists split by the tensors' types."""
+    """``[(type code, tensors, *others)]``: the lists split by the tensors' types."""
     kinds = set(map(_dtype, tensors))
     if not kinds <= _DTYPES.keys():
         raise TypeError(f"{what} takes float32, bfloat16 or float16 tensors, got {kinds - _DTYPES.keys()}")
-    if len(kinds) == 1:
-        return [(*kinds, tensors, *others)]
     keep = {d: [k for k, t in enumerate(tensors) if t.dtype == d] for d in _DTYPES if d in kinds}
-    return [(d, *([x[k] for k in ks] for x in (tensors, *others))) for d, ks in keep.items()]
+    return [(_DTYPES[d], *([x[k] for k in ks] for x in (tensors, *others))) for d, ks in keep.items()]
 
 
-@torch.no_grad()
+def _norm(dev, lists):
+    """The norm of ``lists`` = [(type code, addresses, sizes)] of contiguous tensors on the current device."""
+    lib, stream = _lib.load(), stream_of(dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    size = sum(lib.e2a_grad_norm_workspace_bytes(len(at)) for _, at, _ in lists)
+    ws = torch.empty(max(size, 8), dtype=torch.uint8, device=dev)
+    base, done, count = ws.data_ptr(), 0, array("q", (0,))
+    for code, at, numel in lists:
+        check(lib.e2a_sum_squares(_address(at), _address(numel), len(at), code, base + 8 * done, size - 8 * done,
+                                  _address(count), stream), "e2a_sum_squares")
+        done += count[0]
+    check(lib.e2a_norm_of_squares(base, done, norm.data_ptr(), stream), "e2a_norm_of_squares")
+    return norm
+
+
 def grad_norm(tensors):
     """The global L2 norm ``sqrt(sum of all squares)`` of ``tensors`` (float32, bfloat16 or float16 on one CUDA
     device, any shapes) as a 0-dim float32 tensor there: sums in 64 bits, in a fixed order, no host read.  An
     empty list has norm 0 on the current device."""
-    tensors = _contiguous(list(tensors))
-    dev = _one_device(tensors, "the tensors") if tensors else torch.device("cuda", torch.cuda.current_device())
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return grad_norm(tensors)
-    lib, stream = _lib.load(), stream_of(dev)
-    lists = _by_type("grad_norm", tensors) if tensors else []
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    size = sum(lib.e2a_grad_norm_workspace_bytes(len(ts)) for _, ts in lists)
-    ws = torch.empty(max(size, 8), dtype=torch.uint8, device=dev)
-    at, done, count = ws.data_ptr(), 0, array("q", [0])
-    for dtype, ts in lists:
-        pt, num = _pointers(ts), array("q", map(torch.Tensor.numel, ts))
-        check(lib.e2a_sum_squares(_address(pt), _address(num), len(ts), _DTYPES[dtype], at + 8 * done, size - 8 * done,
-                                  _address(count), stream), "e2a_sum_squares")
-        done += count[0]
-    check(lib.e2a_norm_of_squares(at, done, norm.data_ptr(), stream), "e2a_norm_of_squares")
-    return norm
+    tensors = list(tensors)
+    found = _table(tensors) if tensors else None
+    if found is not None:
+        at, numel, _, code, index = found
+        dev, lists = torch.device("cuda", index), [(code, at, numel)]
+    else:
+        dev = _one_device(tensors, "the tensors") if tensors else torch.device("cuda", torch.cuda.current_device())
+        tensors = _contiguous(tensors)
+        lists = [(code, _pointers(ts), array("q", map(torch.Tensor.numel, ts)))
+                 for code, ts in _by_type("grad_norm", tensors)]
+    if dev.index == torch.cuda.current_device():
+        return _norm(dev, lists)
+    with torch.cuda.device(dev):
+        return _norm(dev, lists)
 
 
 class _Flat:
@@ -235,55 +250,70 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work = []
+        work, keep = [], []
         for gi, g in enumerate(self.param_groups):
-            params = g["params"]
-            grads, index = [p.grad for p in params], None
-            if any(t is None for t in grads):
-                index = [k for k, t in enumerate(grads) if t is not None]
-                params, grads = [params[k] for k in index], [grads[k] for k in index]
-            if grads:
-                work.append((gi, g, params, _contiguous(grads), index))
+            work += self._group_work(gi, g, keep)
+        if not work:
+            return loss
         norm = None
-        if work and self.max_grad_norm is not None:
-            norm = self.last_grad_norm = grad_norm([t for w in work for t in w[3]])
+        if self.max_grad_norm is not None:
+            dev = work[0][1].device
+            if any(w[1].device != dev for w in work):
+                raise ValueError("the parameters to clip together are on more than one device")
+            with torch.cuda.device(dev):
+                norm = self.last_grad_norm = _norm(dev, [(w[2], w[4], w[5]) for w in work])
         for w in work:
-            self._step_group(*w, norm)
+            if w[1].device.index == torch.cuda.current_device():
+                self._launch(*w, norm)
+            else:
+                with torch.cuda.device(w[1].device):
+                    self._launch(*w, norm)
         return loss
 
-    def _step_group(self, gi, group, params, grads, index, norm):
+    def _group_work(self, gi, group, keep):
+        """The launches of a group: ``[(group, flat state, type code, addresses of the parameters and of their
+        gradients, sizes, state offsets, slots, parameters)]``; ``keep`` holds what has to live until then."""
+        params = group["params"]
+        if not params:
+            return []
+        found = _table(params, True)
+        if found is not None:
+            at, numel, grads, code, index = found
+            flat = self._group_state(gi)
+            if index == flat.device.index and numel == flat.numel:
+                return [(group, flat, code, at, grads, numel, flat.offset, flat.slot, params)]
+        index = [k for k, p in enumerate(params) if p.grad is not None]
+        if not index:
+            return []
         flat = self._group_state(gi)
-        dev = flat.device
-        if _one_device(params, "a group's parameters") != dev:
+        params = [params[k] for k in index]
+        if _one_device(params, "a group's parameters") != flat.device:
             raise ValueError("the parameters have moved to another device than their state")
-        if dev.index != torch.cuda.current_device():
-            with torch.cuda.device(dev):
-                return self._step_group(gi, group, params, grads, index, norm)
         if not all(map(torch.Tensor.is_contiguous, params)):
             raise ValueError("AdamW takes contiguous parameters")
-        numel, offset, slot = flat.numel, flat.offset, flat.slot
-        if index is not None:
-            numel, offset, slot = (array(a.typecode, [a[k] for k in index]) for a in (numel, offset, slot))
-        if array("q", map(torch.Tensor.numel, params)) != numel:
+        if any(p.numel() != flat.numel[k] for k, p in zip(index, params)):
             raise ValueError("a parameter has changed its size since its state was made")
+        grads = _contiguous([p.grad for p in params])
+        keep.append(grads)
+        return [(group, flat, code, _pointers(ps), _pointers(gs), *(
+            array(a.typecode, [a[k] for k in ks]) for a in (flat.numel, flat.offset, flat.slot)), ps)
+            for code, ps, gs, ks in _by_type("AdamW", params, grads, index)]
+
+    def _launch(self, group, flat, code, at, grads, numel, offset, slot, params, norm):
         lr, lr_at = group["lr"], None
         if isinstance(lr, torch.Tensor) and lr.is_cuda:
-            if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev:
+            if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != flat.device:
                 raise ValueError("a tensor lr must be one float32 value on the parameters' device")
             lr, lr_at = 0.0, lr.data_ptr()
         (beta1, beta2), b = group["betas"], flat.buffers
-        lib, stream = _lib.load(), stream_of(dev)
         m, v, ms, vs, step = (b[k].data_ptr() if k in b else None for k in (
             "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "step"))
-        for dtype, ps, gs, num, off, slots in _by_type("AdamW", params, grads, numel, offset, slot):
-            num, off, slots = (a if isinstance(a, array) else array(t, a)
-                               for t, a in (("q", num), ("q", off), ("i", slots)))
-            pp, pg = _pointers(ps), _pointers(gs)
-            ws = torch.empty(lib.e2a_adamw_workspace_bytes(len(ps)), dtype=torch.uint8, device=dev)
-            check(lib.e2a_adamw_step(
-                _address(pp), _address(pg), _address(num), _address(off), _address(slots), len(ps), _DTYPES[dtype],
-                flat.bits, m, v, ms, vs, flat.elements, step, lr, lr_at, beta1, beta2, group["eps"],
-                group["weight_decay"], None if norm is None else norm.data_ptr(), self.max_grad_norm or 0.0,
-                ws.data_ptr(), ws.numel(), stream), "e2a_adamw_step")
+        lib = _lib.load()
+        ws = torch.empty(lib.e2a_adamw_workspace_bytes(len(at)), dtype=torch.uint8, device=flat.device)
+        check(lib.e2a_adamw_step(
+            _address(at), _address(grads), _address(numel), _address(offset), _address(slot), len(at), code, flat.bits,
+            m, v, ms, vs, flat.elements, step, lr, lr_at, beta1, beta2, group["eps"], group["weight_decay"],
+            None if norm is None else norm.data_ptr(), self.max_grad_norm or 0.0, ws.data_ptr(), ws.numel(),
+            stream_of(flat.device)), "e2a_adamw_step")
         # the kernels write behind autograd's back: saved tensors and caches keyed on versions have to see it
         torch.autograd.graph.increment_version(params)
