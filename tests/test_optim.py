@@ -1,8 +1,11 @@
 """AdamW over many tensors (32- and 8-bit moments) and the global gradient norm (``ubio_molfm_b200.optim``).
 
-The step's fp32 operations are each rounded once in a stated order, so the reference below, the same order in
-numpy's float32, has to agree bit for bit: in the parameters, the moments and every 8-bit code.  Against the
-formula in 64 bits one step is within a few half steps u = 2^-24 of the terms' magnitudes (see the test)."""
+The moments' fp32 operations are each rounded once in a stated order, so the reference below, the same order in
+numpy's float32, has to agree bit for bit: in 32-bit moments and in every 8-bit code.  The parameter's update takes
+reciprocals and roots within one or two units: with u = 2^-24 the update has relative errors of 2 u (root), u (sum
+with eps), 2 u (reciprocal), u (product) and at most half of the moments', the reference's own about as many, and
+p decay and the difference 2 u each: |dp| <= 16 u (|p| + |update|), and one step of the parameter's type where that
+is narrower (``_same_p``)."""
 import copy
 import ctypes
 import io
@@ -182,6 +185,15 @@ def test_c_abi_refuses_bad_arguments():
 # ------------------------------------------------------------------------------------------------
 # the step
 # ------------------------------------------------------------------------------------------------
+def _same_p(got, before, want, dtype=torch.float32):
+    """``got`` is ``want`` (float32) but for the update's last units; ``before``: the parameter before the step."""
+    up = np.abs(want.astype(np.float64) - before) + 0.2 * np.abs(before)
+    tol = 16 * U * (np.abs(before) + up) + 1e-44
+    if dtype != torch.float32:
+        tol += 2 * HALF[dtype] * np.abs(want) + (2.0 ** -24 if dtype == torch.float16 else 0)
+    return bool((np.abs(got.astype(np.float64) - want) <= tol).all())
+
+
 def _params(sizes, dtype, seed=0):
     gen = torch.Generator().manual_seed(seed)
     ps = []
@@ -224,10 +236,10 @@ def test_steps_equal_the_stated_arithmetic_bit_for_bit(dtype, bits, clip):
             coef = clip_coef(norm, clip)
         for k, (p, r, g) in enumerate(zip(ps, ref, gs)):
             new, m, v = step32(r["p"], g, r["m"], r["v"], t, lr, b1, b2, eps, wd, coef)
-            r["p"] = torch.from_numpy(new).to(dtype).float().numpy()
             st = opt.state[p]
             assert int(st["step"]) == t
-            assert np.array_equal(_np(p), r["p"]), (t, k)
+            assert _same_p(_np(p), r["p"], new, dtype), (t, k)
+            r["p"] = _np(p)
             if bits == 32:
                 r["m"], r["v"] = m, v
                 assert np.array_equal(_np(st["exp_avg"]), m) and np.array_equal(_np(st["exp_avg_sq"]), v), (t, k)
@@ -319,7 +331,7 @@ def test_many_tensors_views_and_unaligned_memory(bits):
     coef = clip_coef(F(math.sqrt(float((g64 ** 2).sum()))), 1.0)
     zero = np.zeros(g64.size, F)
     want, _, _ = step32(_np(before[inside]), g64.astype(F), zero, zero, 1, 1e-2, 0.9, 0.999, 1e-8, 1e-2, coef)
-    assert np.array_equal(_np(p_all[inside]), want)
+    assert _same_p(_np(p_all[inside]), _np(before[inside]), want)
     assert bool((opt.flat_state()["step"] == 1).all())
 
 
@@ -341,7 +353,7 @@ def test_parameters_without_gradient_and_groups():
     assert [int(opt.state[p]["step"]) for p in ps] == [2, 1, 2, 2, 2]
     # the late parameter's first step has its own bias correction: lr g / (|g| + eps), no decay
     want, _, _ = step32(_np(start[1]), np.ones(200, F), np.zeros(200, F), np.zeros(200, F), 1, 1e-3, 0.9, 0.999, 1e-8, 0.0)
-    assert np.array_equal(_np(ps[1]), want)
+    assert _same_p(_np(ps[1]), _np(start[1]), want)
     for p in ps:
         p.grad = None
     opt.step()                                                    # nothing to do
@@ -409,7 +421,7 @@ def test_extreme_magnitudes_in_8_bits():
     om, ov = _offsets(1024, 1)
     (cm, sm), (cv, sv) = pack(m, om, 3), pack(np.sqrt(v), ov, 4)
     st = opt.state[p]
-    assert np.array_equal(_np(p), want)
+    assert _same_p(_np(p), z, want)
     for name, w in (("exp_avg", cm), ("exp_avg_scale", sm), ("exp_avg_sq", cv), ("exp_avg_sq_scale", sv)):
         assert np.array_equal(st[name].cpu().numpy(), w), name
     assert bool(torch.isfinite(torch.stack(opt.moments())).all())

@@ -9,18 +9,19 @@
 // tensor is cut into blocks of 256 elements, its state starts at a multiple of 256 in the group's flat state.
 //
 // 8-bit moments.  The 256 values of a block share a power of two, that of the largest magnitude or the next (one
-// byte, fp32's exponent field; 255 = a value was not finite, the whole block then stands for NaN).  Over it, m is a sign, 4
-// exponent and 3 fraction bits, sqrt(v) 4 exponent and 4 fraction bits, with gradual underflow: the high bits
-// of the fp32 pattern of |x| 2^(-e - 112), whose subnormals fall where the small format's do.  The bits below
+// byte, fp32's exponent field; 255 = a value was not finite, the whole block then stands for NaN).  Over it, m is
+// a sign, 4 exponent and 3 fraction bits, sqrt(v) 4 exponent and 4 fraction bits, with gradual underflow: the high
+// bits of the fp32 pattern of |x| 2^(-e - 112), whose subnormals fall where the small format's do.  The bits below
 // are dropped after adding an offset, mixed bits of (element, step), so a value is rounded up as often as it is
 // near the upper neighbour: round-to-nearest would never move an average whose step is 1 - b2 = 1e-3 of itself
 // (an additive sequence in place of mixed bits locks to the value that it rounds: an average that grows by 1e-3
 // a step fell 6% behind in 2,000 steps).  sqrt(v) > 0 is never rounded to 0 (the update would divide by eps).
-// Every operation is a single rounded fp32 one in a fixed order, so the codes are reproducible bit for bit.
+// The moments' operations are single rounded fp32 ones in a fixed order, so the codes are reproducible bit for bit.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 #include <new>
 #include <type_traits>
 
@@ -72,8 +73,7 @@ __device__ __forceinline__ int tensor_of(const Table& t, int32_t b) {
 // Mixed bits of (element, step): sums and products by odd 32-bit fractions (of the powers of the root of
 // x^5 = x + 1) with shifts between them.  The first moment's offset is the upper 20 bits, the second's the
 // lower 19.
-__device__ __forceinline__ uint32_t mixed(uint32_t i, uint32_t t) {
-  uint32_t u = i * 0xDB4F0B91u + t * 0xBBE05633u;
+__device__ __forceinline__ uint32_t mixed(uint32_t u) {    // u = i 0xDB4F0B91 + t 0xBBE05633
   u = (u ^ (u >> 16)) * 0xA0F2EC75u;
   u = (u ^ (u >> 15)) * 0x89E18285u;
   return u ^ (u >> 16);
@@ -101,7 +101,7 @@ __device__ __forceinline__ float unpack_s(uint32_t code, float scale) {
 __device__ __forceinline__ uint32_t pack_m(float m, uint32_t b, uint32_t dither) {
   if (b == 255u) return 0u;
   const float z = __fmul_rn(__fmul_rn(fabsf(m), __uint_as_float((254u - b) << 23)), two_to_m112());
-  return min((__float_as_uint(z) + dither) >> 20, 127u) | (m < 0.f ? 128u : 0u);
+  return min((__float_as_uint(z) + dither) >> 20, 127u) | ((__float_as_uint(m) >> 24) & 128u);
 }
 __device__ __forceinline__ uint32_t pack_s(float s, uint32_t b, uint32_t dither) {
   if (b == 255u) return 0u;
@@ -111,7 +111,7 @@ __device__ __forceinline__ uint32_t pack_s(float s, uint32_t b, uint32_t dither)
 
 // ---- the step ------------------------------------------------------------------------------------
 struct Hyper {
-  double lr, beta1, beta2, decay;
+  double lr, log_beta1, log_beta2, decay;    // the betas' logarithms to base 2
   const float* lr_dev;
   const float* norm;
   float max_norm;
@@ -132,8 +132,8 @@ __global__ void k_adamw_scalars(const __grid_constant__ Slots slots, Hyper h, in
     const int32_t t = step[k] + 1;
     if (!skip) step[k] = t;
     Scalars v;
-    v.size = (float)(lr / (1.0 - pow(h.beta1, (double)t)));
-    v.root = (float)(1.0 / sqrt(1.0 - pow(h.beta2, (double)t)));
+    v.size = (float)(lr / (1.0 - exp2(t * h.log_beta1)));
+    v.root = (float)(1.0 / sqrt(1.0 - exp2(t * h.log_beta2)));
     v.t = t;
     v.pad = 0;
     s[j] = v;
@@ -148,18 +148,30 @@ __global__ void k_adamw_scalars(const __grid_constant__ Slots slots, Hyper h, in
   }
 }
 
-struct Moments { float p, m, v; };
+__device__ __forceinline__ float reciprocal(float x) {      // within 1 unit; 0 for inf, inf below 2^-126
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float root_approx(float x) {     // within 2^-23; 0 below 2^-126
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
-// One element's update; every operation rounded on its own (see above).
-__device__ __forceinline__ Moments update(float p, float g, float m, float v, const Globals& gl, const Scalars& s,
-                                          float b1, float a1, float b2, float a2, float eps, bool clip) {
-  if (clip) g = __fmul_rn(g, gl.coef);
-  Moments o;
-  o.m = __fadd_rn(__fmul_rn(m, b1), __fmul_rn(g, a1));
-  o.v = __fadd_rn(__fmul_rn(v, b2), __fmul_rn(__fmul_rn(g, g), a2));
-  const float d = __fadd_rn(__fmul_rn(__fsqrt_rn(o.v), s.root), eps);
-  o.p = __fsub_rn(__fmul_rn(p, gl.decay), __fmul_rn(__fdiv_rn(o.m, d), s.size));
-  return o;
+// What all elements of a launch share.
+struct Rates { float b1, a1, b2, a2, eps; };
+
+// One element's moments; every operation rounded on its own (see above).
+__device__ __forceinline__ float next_m(float m, float g, const Rates& r) {
+  return __fadd_rn(__fmul_rn(m, r.b1), __fmul_rn(g, r.a1));
+}
+__device__ __forceinline__ float next_v(float v, float g, const Rates& r) {
+  return __fadd_rn(__fmul_rn(v, r.b2), __fmul_rn(__fmul_rn(g, g), r.a2));
+}
+// p decay - m / (s root + eps) size: nothing is kept of it but p, so the quotient may be a unit or two off.
+__device__ __forceinline__ float next_p(float p, float m, float s, const Globals& gl, const Scalars& sc, float eps) {
+  return fmaf(-m * reciprocal(fmaf(s, sc.root, eps)), sc.size, p * gl.decay);
 }
 
 // Four neighbouring values of a tensor of n from element i on, 0 beyond its end; one load where the tensor's
@@ -194,14 +206,127 @@ __device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, flo
   }
 }
 
-// A CTA walks a contiguous range of units, 8 values a thread and unit: a warp owns one block of 256, lane l the
-// values 4 l and 128 + 4 l on (16-byte loads of fp32, 4-byte ones of codes, all neighbouring).
+// Eight values of a thread: elements 4 l and 128 + 4 l on of its warp's block.
+struct Eight { float v[8]; };
+
+template <typename T>
+__device__ __forceinline__ Eight load8(const T* p, int64_t i, int64_t n, bool vec) {
+  Eight o;
+  *reinterpret_cast<float4*>(o.v) = load4(p, i, n, vec);
+  *reinterpret_cast<float4*>(o.v + 4) = load4(p, i + 128, n, vec);
+  return o;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int64_t i, int64_t n, bool vec, const Eight& v) {
+  store4(p, i, n, vec, *reinterpret_cast<const float4*>(v.v));
+  store4(p, i + 128, n, vec, *reinterpret_cast<const float4*>(v.v + 4));
+}
+
+// Where a warp's block lies and what its tensor shares.
+struct Where {
+  int64_t i, n;        // the thread's first element, the tensor's elements
+  uint32_t mix;        // i and t's share of the mixed bits
+};
+
+constexpr uint32_t kMixIndex = 0xDB4F0B91u;
+
+// A thread's share of a block: parameters, codes and shared exponents.
+struct Held {
+  Eight p;
+  uint32_t cm[2], cv[2], em, es;
+};
+
+// The step for any values.  By value: the arguments of the rarely made call must not tie the caller's to memory.
+__device__ __noinline__ Held block_exact(const Held h, const Eight g, const Where w, const Globals gl, const Scalars sc,
+                                         const Rates r) {
+  Held o;
+  Eight m, s;
+  uint32_t top_m = 0, top_s = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float r0 = unpack_s((h.cv[e / 4] >> (8 * (e % 4))) & 255u, scale_of(h.es));
+    m.v[e] = next_m(unpack_m((h.cm[e / 4] >> (8 * (e % 4))) & 255u, scale_of(h.em)), g.v[e], r);
+    s.v[e] = __fsqrt_rn(next_v(__fmul_rn(r0, r0), g.v[e], r));
+    o.p.v[e] = next_p(h.p.v[e], m.v[e], s.v[e], gl, sc, r.eps);
+    if (w.i + e % 4 + 128 * (e / 4) >= w.n) m.v[e] = s.v[e] = 0.f;     // a block holds no more than its tensor
+    top_m = max(top_m, __float_as_uint(m.v[e]) & 0x7FFFFFFFu);
+    top_s = max(top_s, __float_as_uint(s.v[e]) & 0x7FFFFFFFu);
+  }
+  o.em = shared_exponent(__reduce_max_sync(0xffffffffu, top_m), 3);
+  o.es = shared_exponent(__reduce_max_sync(0xffffffffu, top_s), 4);
+  o.cm[0] = o.cm[1] = o.cv[0] = o.cv[1] = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t u = mixed(w.mix + (e % 4 + 128 * (e / 4)) * kMixIndex);
+    o.cm[e / 4] |= pack_m(m.v[e], o.em, u >> 12) << (8 * (e % 4));
+    o.cv[e / 4] |= pack_s(s.v[e], o.es, u & 0x7FFFFu) << (8 * (e % 4));
+  }
+  return o;
+}
+
+// The same codes for a whole block of ordinary values in about half the instructions: scales as one product, no
+// clamps, and square roots within 2^-23, whose code is the exact root's unless the rounding offset brings it within
+// a few units of the next one.  False (for all of the warp) where any of this may not hold: block_exact then does
+// it again from h.
+__device__ __forceinline__ bool block_fast(const Held& h, Held& o, const Eight& g, const Where& w, const Globals& gl,
+                                           const Scalars& sc, const Rates& r) {
+  // scales 2^(e + 112) of the old codes, in range for e <= 15; none for a NaN block
+  if (w.i - 4 * (threadIdx.x & 31) + kBlock > w.n || max(h.em, h.es) > 127 + 15) return false;
+  const float fm = __uint_as_float((h.em + 112u) << 23), fs = __uint_as_float((h.es + 112u) << 23);
+  Eight m, s;
+  uint32_t top_m = 0, top_s = 0, alive = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int k = 8 * (e % 4);
+    const uint32_t a = h.cm[e / 4], b = h.cv[e / 4];
+    // magnitude to bits 20..26, sign to bit 31
+    const uint32_t mag = (k <= 20 ? a << (20 - k) : a >> (k - 20)) & 0x07F00000u, sign = (a << (24 - k)) & 0x80000000u;
+    const float m0 = __fmul_rn(__uint_as_float(mag | sign), fm);
+    const float s0 = __fmul_rn(__uint_as_float((k <= 19 ? b << (19 - k) : b >> (k - 19)) & 0x07F80000u), fs);
+    m.v[e] = next_m(m0, g.v[e], r);
+    const float v = next_v(__fmul_rn(s0, s0), g.v[e], r);
+    alive |= (__float_as_uint(v) != 0u ? 1u : 0u) << e;
+    s.v[e] = root_approx(v);
+    o.p.v[e] = next_p(h.p.v[e], m.v[e], s.v[e], gl, sc, r.eps);
+    top_m = max(top_m, __float_as_uint(m.v[e]) & 0x7FFFFFFFu);
+    top_s = max(top_s, __float_as_uint(s.v[e]));
+  }
+  top_m = __reduce_max_sync(0xffffffffu, top_m);
+  top_s = __reduce_max_sync(0xffffffffu, top_s);
+  const uint32_t em = shared_exponent(top_m, 3), es = shared_exponent(top_s, 4);
+  // in range for one product each (NaN and infinities are above), and the exponent not in doubt
+  if (em > 127 + 14 || es > 127 + 14 || es < 127 - 40 || ((top_s + (1u << 19) + 4u) & 0x7FFFFFu) < 8u) return false;
+  const float zm = __uint_as_float((254u - 112u - em) << 23), zs = __uint_as_float((254u - 112u - es) << 23);
+  uint32_t wm[2] = {0, 0}, ws[2] = {0, 0}, doubt = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int k = 8 * (e % 4);
+    const uint32_t u = mixed(w.mix + (e % 4 + 128 * (e / 4)) * kMixIndex);
+    const uint32_t bm = __float_as_uint(m.v[e]);
+    const uint32_t tm = __float_as_uint(__fmul_rn(fabsf(m.v[e]), zm)) + (u >> 12);
+    wm[e / 4] |= (tm >> 20) << k | ((bm >> 24) & 128u) << k;
+    const uint32_t ts = __float_as_uint(__fmul_rn(s.v[e], zs)) + (u & 0x7FFFFu);
+    doubt |= ((ts + 4u) & 0x7FFFFu) < 8u ? 1u : 0u;
+    ws[e / 4] |= max(ts >> 19, (alive >> e) & 1u) << k;
+  }
+  if (__any_sync(0xffffffffu, doubt)) return false;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    o.cm[k] = wm[k];
+    o.cv[k] = ws[k];
+  }
+  o.em = em;
+  o.es = es;
+  return true;
+}
+
+// A CTA walks a contiguous range of units; a warp owns one block of 256 of each, lane l the values 4 l and
+// 128 + 4 l on (16-byte loads of fp32, 4-byte ones of codes, all neighbouring).
 template <typename T, int BITS>
 __global__ void __launch_bounds__(kThreads)
 k_adamw(const __grid_constant__ Table tab, int32_t n_units, int32_t per_cta, void* __restrict__ exp_avg,
         void* __restrict__ exp_avg_sq, uint8_t* __restrict__ scale_m, uint8_t* __restrict__ scale_v,
-        const Scalars* __restrict__ scal, const Globals* __restrict__ glob, float b1, float a1, float b2, float a2,
-        float eps, bool clip) {
+        const Scalars* __restrict__ scal, const Globals* __restrict__ glob, const Rates r, bool clip) {
   const Globals gl = *glob;
   if (gl.skip) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -211,90 +336,52 @@ k_adamw(const __grid_constant__ Table tab, int32_t n_units, int32_t per_cta, voi
     while (b >= tab.first[j + 1]) ++j;
     const int64_t i0 = (int64_t)(b - tab.first[j]) * kUnit + warp * kBlock, n = tab.numel[j];
     if (i0 >= n) continue;
-    const int64_t at = tab.offset[j] + i0;
+    const int64_t i = i0 + 4 * lane, at = tab.offset[j] + i;
     const Scalars s = scal[j];
-    T* p = reinterpret_cast<T*>(tab.p[j]);
-    const T* g = reinterpret_cast<const T*>(tab.g[j]);
+    T* pt = reinterpret_cast<T*>(tab.p[j]);
     const bool vec = ((tab.p[j] | tab.g[j]) & (4 * sizeof(T) - 1)) == 0;
-    float4 pv[2], gv[2], mv[2], vv[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int c = 4 * lane + 128 * k;
-      pv[k] = load4(p, i0 + c, n, vec);
-      gv[k] = load4(g, i0 + c, n, vec);
-    }
-    uint32_t cm[2], cv[2];
-    float sm = 0.f, ss = 0.f;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int c = 4 * lane + 128 * k;
-      if (BITS == 32) {
-        mv[k] = *reinterpret_cast<const float4*>((const float*)exp_avg + at + c);
-        vv[k] = *reinterpret_cast<const float4*>((const float*)exp_avg_sq + at + c);
-      } else {
-        cm[k] = *reinterpret_cast<const uint32_t*>((const uint8_t*)exp_avg + at + c);
-        cv[k] = *reinterpret_cast<const uint32_t*>((const uint8_t*)exp_avg_sq + at + c);
-      }
-    }
-    if (BITS == 8) {
-      sm = scale_of(scale_m[at / kBlock]);
-      ss = scale_of(scale_v[at / kBlock]);
-    }
-    uint32_t top_m = 0, top_s = 0;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float* pe = reinterpret_cast<float*>(&pv[k]);
-      float* me = reinterpret_cast<float*>(&mv[k]);
-      float* ve = reinterpret_cast<float*>(&vv[k]);
-      const float* ge = reinterpret_cast<const float*>(&gv[k]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (BITS == 8) {
-          me[e] = unpack_m((cm[k] >> (8 * e)) & 255u, sm);
-          const float r = unpack_s((cv[k] >> (8 * e)) & 255u, ss);
-          ve[e] = __fmul_rn(r, r);
-        }
-        const Moments o = update(pe[e], ge[e], me[e], ve[e], gl, s, b1, a1, b2, a2, eps, clip);
-        pe[e] = o.p;
-        me[e] = o.m;
-        ve[e] = o.v;
-        if (BITS == 8) {
-          if (i0 + 4 * lane + 128 * k + e >= n) me[e] = ve[e] = 0.f;   // a NaN block holds no more than its tensor
-          ve[e] = __fsqrt_rn(ve[e]);
-          top_m = max(top_m, __float_as_uint(me[e]) & 0x7FFFFFFFu);
-          top_s = max(top_s, __float_as_uint(ve[e]) & 0x7FFFFFFFu);
-        }
-      }
-      store4(p, i0 + 4 * lane + 128 * k, n, vec, pv[k]);
-    }
+    Eight p = load8(pt, i, n, vec), g = load8(reinterpret_cast<const T*>(tab.g[j]), i, n, vec);
     if (BITS == 32) {
+      float* mt = (float*)exp_avg + at;
+      float* vt = (float*)exp_avg_sq + at;
+      Eight m, v;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int c = 4 * lane + 128 * k;
-        *reinterpret_cast<float4*>((float*)exp_avg + at + c) = mv[k];
-        *reinterpret_cast<float4*>((float*)exp_avg_sq + at + c) = vv[k];
+        *reinterpret_cast<float4*>(m.v + 4 * k) = *reinterpret_cast<const float4*>(mt + 128 * k);
+        *reinterpret_cast<float4*>(v.v + 4 * k) = *reinterpret_cast<const float4*>(vt + 128 * k);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (clip) g.v[e] = __fmul_rn(g.v[e], gl.coef);
+        m.v[e] = next_m(m.v[e], g.v[e], r);
+        v.v[e] = next_v(v.v[e], g.v[e], r);
+        p.v[e] = next_p(p.v[e], m.v[e], __fsqrt_rn(v.v[e]), gl, s, r.eps);
+      }
+      store8(pt, i, n, vec, p);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        *reinterpret_cast<float4*>(mt + 128 * k) = *reinterpret_cast<const float4*>(m.v + 4 * k);
+        *reinterpret_cast<float4*>(vt + 128 * k) = *reinterpret_cast<const float4*>(v.v + 4 * k);
       }
     } else {
-      const uint32_t em = shared_exponent(__reduce_max_sync(0xffffffffu, top_m), 3);
-      const uint32_t es = shared_exponent(__reduce_max_sync(0xffffffffu, top_s), 4);
+      uint32_t* mt = reinterpret_cast<uint32_t*>((uint8_t*)exp_avg + at);
+      uint32_t* vt = reinterpret_cast<uint32_t*>((uint8_t*)exp_avg_sq + at);
+      const Held h{p, {mt[0], mt[32]}, {vt[0], vt[32]}, scale_m[at / kBlock], scale_v[at / kBlock]};
+      Held o;
+      if (clip) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int c = 4 * lane + 128 * k;
-        const float* me = reinterpret_cast<const float*>(&mv[k]);
-        const float* ve = reinterpret_cast<const float*>(&vv[k]);
-        uint32_t wm = 0, ws = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t u = mixed((uint32_t)(i0 + c + e), (uint32_t)s.t);
-          wm |= pack_m(me[e], em, u >> 12) << (8 * e);
-          ws |= pack_s(ve[e], es, u & 0x7FFFFu) << (8 * e);
-        }
-        *reinterpret_cast<uint32_t*>((uint8_t*)exp_avg + at + c) = wm;
-        *reinterpret_cast<uint32_t*>((uint8_t*)exp_avg_sq + at + c) = ws;
+        for (int e = 0; e < 8; ++e) g.v[e] = __fmul_rn(g.v[e], gl.coef);
       }
+      const Where w{i, n, (uint32_t)i * kMixIndex + (uint32_t)s.t * 0xBBE05633u};
+      if (!block_fast(h, o, g, w, gl, s, r)) o = block_exact(h, g, w, gl, s, r);
+      store8(pt, i, n, vec, o.p);
+      mt[0] = o.cm[0];
+      mt[32] = o.cm[1];
+      vt[0] = o.cv[0];
+      vt[32] = o.cv[1];
       if (lane == 0) {
-        scale_m[at / kBlock] = (uint8_t)em;
-        scale_v[at / kBlock] = (uint8_t)es;
+        scale_m[at / kBlock] = (uint8_t)o.em;
+        scale_v[at / kBlock] = (uint8_t)o.es;
       }
     }
   }
@@ -320,7 +407,7 @@ k_moments_unpack(const uint8_t* __restrict__ m, const uint8_t* __restrict__ v, c
   }
 }
 
-// ---- the global norm -------------------------------------------------------------------------------
+// ---- the global norm: partial sums in 64 bits, added up in order -----------------------------------
 __device__ __forceinline__ double cta_sum(double s, double* sh) {
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
@@ -330,12 +417,36 @@ __device__ __forceinline__ double cta_sum(double s, double* sh) {
   return s;
 }
 
-// Squares are exact in 64 bits and summed there: the norm is the correctly rounded one but for ties.
+// The sum of eight squares in 64 bits, where every product is exact and the sum as good as.  An fp32 value's bits
+// are those of the 64-bit one but for the exponent's bias (896 more) and its place, which two or three integer
+// operations do faster than the conversion unit (240M bf16 values: 131 us with conversions).  That holds for
+// ordinary values: zeros and subnormals come out as at most 2^-126, which a sum over 1e-20 does not see.  Other
+// groups, with infinities and NaN among them, are converted.
+__device__ __forceinline__ double squares(const float4 a, const float4 b) {
+  const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  float rough = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) rough = fmaf(v[k], v[k], rough);
+  double d[2] = {0., 0.};
+  if (rough > 1e-20f && rough < 1e38f) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t bits = __float_as_uint(v[k]) & 0x7FFFFFFFu;
+      const double x = __hiloint2double((int)((bits >> 3) + (896u << 20)), (int)(bits << 29));
+      d[k & 1] = fma(x, x, d[k & 1]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) d[k & 1] = fma((double)v[k], (double)v[k], d[k & 1]);
+  }
+  return d[0] + d[1];
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 k_sum_squares(const __grid_constant__ Table tab, int32_t n_units, int32_t per_cta, double* __restrict__ part) {
   __shared__ double sh[kThreads / 32];
-  double s[2] = {0., 0.};
+  double s = 0.;
   const int32_t from = blockIdx.x * per_cta, to = min(from + per_cta, n_units);
   int j = tensor_of(tab, from);
   for (int32_t b = from; b < to; ++b) {
@@ -343,18 +454,9 @@ k_sum_squares(const __grid_constant__ Table tab, int32_t n_units, int32_t per_ct
     const int64_t i0 = (int64_t)(b - tab.first[j]) * kUnit, n = tab.numel[j];
     const T* g = reinterpret_cast<const T*>(tab.g[j]);
     const bool vec = (tab.g[j] & (4 * sizeof(T) - 1)) == 0;
-    float4 v[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) v[k] = load4(g, i0 + 4 * (threadIdx.x + kThreads * k), n, vec);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      s[0] = fma((double)v[k].x, (double)v[k].x, s[0]);
-      s[1] = fma((double)v[k].y, (double)v[k].y, s[1]);
-      s[0] = fma((double)v[k].z, (double)v[k].z, s[0]);
-      s[1] = fma((double)v[k].w, (double)v[k].w, s[1]);
-    }
+    s += squares(load4(g, i0 + 4 * threadIdx.x, n, vec), load4(g, i0 + 4 * (threadIdx.x + kThreads), n, vec));
   }
-  const double all = cta_sum(s[0] + s[1], sh);
+  const double all = cta_sum(s, sh);
   if (threadIdx.x == 0) part[blockIdx.x] = all;
 }
 
@@ -506,8 +608,8 @@ int e2a_adamw_step(const uint64_t* params, const uint64_t* grads, const int64_t*
   Globals* glob = (Globals*)workspace;
   Scalars* scal = (Scalars*)(glob + 1);
   cudaStream_t st = (cudaStream_t)stream;
-  const Hyper h{lr, beta1, beta2, weight_decay, lr_device, grad_norm, (float)max_norm};
-  const float b1 = (float)beta1, a1 = (float)(1. - beta1), b2 = (float)beta2, a2 = (float)(1. - beta2);
+  const Hyper h{lr, std::log2(beta1), std::log2(beta2), weight_decay, lr_device, grad_norm, (float)max_norm};
+  const Rates r{(float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps};
   for (int64_t j = 0; j < n_tensors;) {
     static thread_local Table t;
     static thread_local Slots slot;
@@ -523,7 +625,7 @@ int e2a_adamw_step(const uint64_t* params, const uint64_t* grads, const int64_t*
       auto* kernel = state_bits == 32 ? k_adamw<T, 32> : k_adamw<T, 8>;
       const int32_t per = (units + kStepCtas - 1) / kStepCtas, ctas = (units + per - 1) / per;
       kernel<<<ctas, kThreads, 0, st>>>(t, units, per, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale,
-                                        scal + from, glob, b1, a1, b2, a2, (float)eps, grad_norm != nullptr);
+                                        scal + from, glob, r, grad_norm != nullptr);
       E2A_CHECK_LAUNCH();
       return E2A_OK;
     });
