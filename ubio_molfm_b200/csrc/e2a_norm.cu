@@ -16,6 +16,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "e2a_common.cuh"
@@ -44,6 +45,43 @@ __device__ __forceinline__ Act activation(float z, bool silu) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.44269504f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
   return {z * s, s * (1.f + z * (1.f - s)), s * (1.f - s) * (2.f + z * (1.f - 2.f * s))};
+}
+
+// The same of two neighbouring values: packed fp32 arithmetic takes one issue slot for both.
+__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 f2_mul(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 f2_add(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 sigmoid(float2 z) {
+  const float2 t = f2_mul(z, f2(-1.44269504f));
+  float2 e, s;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  e = f2_add(e, f2(1.f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(e.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(e.y));
+  return s;
+}
+struct Act2 { float2 d1, d2; };
+template <bool SILU, bool SECOND>
+__device__ __forceinline__ Act2 derivatives(float2 z) {
+  if (!SILU) return {f2(1.f), f2(0.f)};
+  const float2 s = sigmoid(z), rest = f2_fma(s, f2(-1.f), f2(1.f));
+  Act2 a;
+  a.d1 = f2_mul(s, f2_fma(z, rest, f2(1.f)));
+  a.d2 = SECOND ? f2_mul(f2_mul(s, rest), f2_fma(z, f2_fma(s, f2(-2.f), f2(1.f)), f2(2.f))) : f2(0.f);
+  return a;
 }
 
 struct Norm {
@@ -220,22 +258,19 @@ __global__ void k_ln_cols_sum(const double* __restrict__ part, int64_t chunks, i
 
 // ------------------------------------------------------------------------------------------------
 // Rows in registers.  A team of TEAM threads holds a row, VEC neighbouring values (16 bytes, or one where the
-// strides or addresses allow no more) V times a thread, and RB rows at a time so that enough loads are in flight.
-// Teams of at most a warp share a CTA of 256 threads and meet only in shuffles; wider rows take a CTA each.
+// strides or addresses allow no more) V times a thread; the next row's loads are issued before the current one is
+// worked on, so they are in flight all the time.  Teams of at most a warp share a CTA of 256 threads and meet only
+// in shuffles; wider rows take a CTA each.
 // ------------------------------------------------------------------------------------------------
 template <typename T, int VEC> struct Pack;
 template <> struct Pack<float, 4> {
-  static __device__ __forceinline__ void load(const float* p, float* v) {
-    const float4 t = ldg4(p);
-    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-  }
-  static __device__ __forceinline__ void store(float* p, const float* v) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  }
+  using Raw = float4;
+  static __device__ __forceinline__ void widen(const Raw& t, float* v) { v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w; }
+  static __device__ __forceinline__ Raw narrow(const float* v) { return make_float4(v[0], v[1], v[2], v[3]); }
 };
 template <typename T, typename T2> struct Pack16 {
-  static __device__ __forceinline__ void load(const T* p, float* v) {
-    const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
+  using Raw = uint4;
+  static __device__ __forceinline__ void widen(const Raw& t, float* v) {
     const uint32_t w[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -244,7 +279,7 @@ template <typename T, typename T2> struct Pack16 {
       v[2 * i + 1] = to_f(h.y);
     }
   }
-  static __device__ __forceinline__ void store(T* p, const float* v) {
+  static __device__ __forceinline__ Raw narrow(const float* v) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -253,14 +288,15 @@ template <typename T, typename T2> struct Pack16 {
       h.y = from_f<T>(v[2 * i + 1]);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 template <> struct Pack<__nv_bfloat16, 8> : Pack16<__nv_bfloat16, __nv_bfloat162> {};
 template <> struct Pack<__half, 8> : Pack16<__half, __half2> {};
 template <typename T> struct Pack<T, 1> {
-  static __device__ __forceinline__ void load(const T* p, float* v) { v[0] = to_f(p[0]); }
-  static __device__ __forceinline__ void store(T* p, const float* v) { p[0] = from_f<T>(v[0]); }
+  using Raw = T;
+  static __device__ __forceinline__ void widen(const Raw& t, float* v) { v[0] = to_f(t); }
+  static __device__ __forceinline__ Raw narrow(const float* v) { return from_f<T>(v[0]); }
 };
 
 // fp32 vectors of the affine parameters: VEC at a time in 16-byte loads (they come from fresh or parameter
@@ -309,92 +345,124 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float* sh, int& turn) {
   }
 }
 
-template <typename T_, int VEC_, int V_, int TEAM_, int RB_>
+template <typename T_, int VEC_, int V_, int TEAM_>
 struct Shape {
   using T = T_;
-  static constexpr int VEC = VEC_, V = V_, TEAM = TEAM_, RB = RB_;
-  static constexpr int THREADS = TEAM > 256 ? TEAM : (TEAM > 32 ? TEAM : 256);
-  static constexpr int TEAMS = THREADS / TEAM;   // rows that a CTA holds at a time, times RB
+  using P = Pack<T, VEC_>;
+  static constexpr int VEC = VEC_, V = V_, TEAM = TEAM_;
+  static constexpr int THREADS = TEAM > 32 ? TEAM : 256;
+  static constexpr int TEAMS = THREADS / TEAM;   // rows that a CTA holds at a time
   static constexpr int N = VEC * V;
-  static constexpr int COLS = N * TEAM;
+  static constexpr int SCRATCH = TEAM > 32 ? 2 * 5 * (TEAM / 32) : 1;                    // team_sum
 };
 
+// The rows a thread works on, of K operands at once, one row ahead of their use in registers.  (Two to four rows
+// ahead in shared memory by asynchronous copies took 3 to 15% longer at every shape tried.)
+template <class S, int K>
+struct Rows {
+  using T = typename S::T;
+  using Raw = typename S::P::Raw;
+  const T* p[K];
+  int64_t ld[K], rows, step;
+  int W;
+  Raw next[K][S::V];
+
+  __device__ __forceinline__ void load(int64_t row) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int i = 0; i < S::V; ++i) {
+        const int c = (threadIdx.x % S::TEAM + S::TEAM * i) * S::VEC;
+        next[k][i] = row < rows && c < W ? __ldg(reinterpret_cast<const Raw*>(p[k] + row * ld[k] + c)) : Raw{};
+      }
+    }
+  }
+  // The values of `row` (zero beyond the rows' and the row's end), the next row's on their way.
+  __device__ __forceinline__ void take(int64_t row, float (&v)[K][S::N]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int i = 0; i < S::V; ++i) S::P::widen(next[k][i], v[k] + i * S::VEC);
+    }
+    load(row + step);
+  }
+};
+
+// A thread's values as pairs.  The vectors' own pairs with 16-byte loads, neighbours of its V single ones without.
+#define E2A_PAIR(v, e) (reinterpret_cast<float2*>(v)[e])
+
+// gamma, beta, p, q at a thread's columns, `without` beyond the row's end too.
 template <class S>
+__device__ __forceinline__ void columns(const float* p, int W, float without, float (&v)[S::N]) {
+#pragma unroll
+  for (int i = 0; i < S::V; ++i) {
+    const int c = (threadIdx.x % S::TEAM + S::TEAM * i) * S::VEC;
+    load_affine<S::VEC>(c < W ? p : nullptr, c, without, v + i * S::VEC);
+  }
+}
+
+template <class S, bool SILU>
 __global__ void __launch_bounds__(S::THREADS)
 k_row_fwd(const typename S::T* __restrict__ x, int64_t ldx, Norm n, int64_t rows, float eps,
           typename S::T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-  using P = Pack<typename S::T, S::VEC>;
-  __shared__ float sh[S::TEAM > 32 ? 2 * 5 * (S::TEAM / 32) : 1];
+  using Raw = typename S::P::Raw;
+  __shared__ float sh[S::SCRATCH];
   int turn = 0;
-  const int me = threadIdx.x % S::TEAM, team = threadIdx.x / S::TEAM, W = (int)n.W;
+  const int me = threadIdx.x % S::TEAM, W = (int)n.W;
+  const int64_t step = gridDim.x * (int64_t)S::TEAMS;
   const float inv = 1.f / W;
-  for (int64_t base = blockIdx.x * (int64_t)(S::TEAMS * S::RB); base < rows;
-       base += gridDim.x * (int64_t)(S::TEAMS * S::RB)) {
-    float v[S::RB][S::N];
-    int64_t row[S::RB];
+  int64_t row = blockIdx.x * (int64_t)S::TEAMS + threadIdx.x / S::TEAM;
+  Rows<S, 1> in{{x}, {ldx}, rows, step, W};
+  in.load(row);
+  for (int64_t base = blockIdx.x * (int64_t)S::TEAMS; base < rows; base += step, row += step) {
+    alignas(8) float v[1][S::N];
+    in.take(row, v);
+    float2 two = f2(0.f);
 #pragma unroll
-    for (int b = 0; b < S::RB; ++b) {
-      row[b] = base + b * S::TEAMS + team;
+    for (int e = 0; e < S::N / 2; ++e) two = f2_add(two, E2A_PAIR(v[0], e));
+    float sum[1] = {two.x + two.y};
+    team_sum<S::TEAM>(sum, sh, turn);
+    const float mean = sum[0] * inv;
+    two = f2(0.f);
 #pragma unroll
-      for (int i = 0; i < S::V; ++i) {
-        const int c = (me + S::TEAM * i) * S::VEC;
-        if (row[b] < rows && c < W) {
-          P::load(x + row[b] * ldx + c, v[b] + i * S::VEC);
-        } else {
+    for (int i = 0; i < S::V; ++i) {
+      if ((me + S::TEAM * i) * S::VEC >= W) {       // beyond the row's end: as if it were the mean
 #pragma unroll
-          for (int k = 0; k < S::VEC; ++k) v[b][i * S::VEC + k] = 0.f;
-        }
+        for (int k = 0; k < S::VEC; ++k) v[0][i * S::VEC + k] = mean;
       }
     }
-    float mean[S::RB], var[S::RB];
 #pragma unroll
-    for (int b = 0; b < S::RB; ++b) {
-      mean[b] = 0.f;
-#pragma unroll
-      for (int k = 0; k < S::N; ++k) mean[b] += v[b][k];
+    for (int e = 0; e < S::N / 2; ++e) {
+      E2A_PAIR(v[0], e) = f2_add(E2A_PAIR(v[0], e), f2(-mean));
+      two = f2_fma(E2A_PAIR(v[0], e), E2A_PAIR(v[0], e), two);
     }
-    team_sum<S::TEAM>(mean, sh, turn);
-#pragma unroll
-    for (int b = 0; b < S::RB; ++b) {
-      mean[b] *= inv;
-      var[b] = 0.f;
-#pragma unroll
-      for (int i = 0; i < S::V; ++i) {
-        if ((me + S::TEAM * i) * S::VEC < W) {
-#pragma unroll
-          for (int k = 0; k < S::VEC; ++k) {
-            float& t = v[b][i * S::VEC + k];
-            t -= mean[b];
-            var[b] += t * t;
-          }
-        }
-      }
+    sum[0] = two.x + two.y;
+    constexpr bool EARLY = S::TEAM > 32 || S::N <= 8;     // beside the sum, where registers allow
+    alignas(8) float ga[S::N], be[S::N];
+    if (EARLY) {
+      columns<S>(n.gamma, W, 1.f, ga);
+      columns<S>(n.beta, W, 0.f, be);
     }
-    team_sum<S::TEAM>(var, sh, turn);
+    team_sum<S::TEAM>(sum, sh, turn);
+    const float rstd = rsqrtf(sum[0] * inv + eps);
+    if (row >= rows) continue;      // a team of a warp or less: the others go on; a CTA's rows all exist
+    if (me == 0) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+    if (!EARLY) {
+      columns<S>(n.gamma, W, 1.f, ga);
+      columns<S>(n.beta, W, 0.f, be);
+    }
 #pragma unroll
-    for (int b = 0; b < S::RB; ++b) {
-      var[b] = rsqrtf(var[b] * inv + eps);      // rstd
-      if (me == 0 && row[b] < rows) {
-        mean_out[row[b]] = mean[b];
-        rstd_out[row[b]] = var[b];
-      }
+    for (int e = 0; e < S::N / 2; ++e) {
+      const float2 z = f2_fma(f2_mul(E2A_PAIR(v[0], e), f2(rstd)), E2A_PAIR(ga, e), E2A_PAIR(be, e));
+      E2A_PAIR(v[0], e) = SILU ? f2_mul(z, sigmoid(z)) : z;
     }
 #pragma unroll
     for (int i = 0; i < S::V; ++i) {
       const int c = (me + S::TEAM * i) * S::VEC;
-      if (c < W) {
-        float ga[S::VEC], be[S::VEC];
-        load_affine<S::VEC>(n.gamma, c, 1.f, ga);
-        load_affine<S::VEC>(n.beta, c, 0.f, be);
-#pragma unroll
-        for (int b = 0; b < S::RB; ++b) {
-          float o[S::VEC];
-#pragma unroll
-          for (int k = 0; k < S::VEC; ++k)
-            o[k] = activation(v[b][i * S::VEC + k] * var[b] * ga[k] + be[k], n.silu).y;
-          if (row[b] < rows) P::store(y + row[b] * W + c, o);
-        }
-      }
+      if (c < W) *reinterpret_cast<Raw*>(y + row * W + c) = S::P::narrow(v[0] + i * S::VEC);
     }
   }
 }
@@ -423,21 +491,21 @@ __device__ __forceinline__ void flush_cols(float (&dw)[S::N], float (&db)[S::N],
 #pragma unroll
         for (int k = 0; k < S::N; ++k) d[k] += __shfl_xor_sync(0xffffffffu, d[k], o);
       }
-      constexpr int WARPS = S::THREADS / 32;
+      constexpr int WARPS = S::THREADS / 32, COLS = S::TEAM * S::N;
       __syncthreads();
       if ((threadIdx.x & 31) < S::TEAM) {
 #pragma unroll
         for (int i = 0; i < S::V; ++i) {
 #pragma unroll
           for (int k = 0; k < S::VEC; ++k)
-            sh[(threadIdx.x >> 5) * S::COLS + (me + S::TEAM * i) * S::VEC + k] = d[i * S::VEC + k];
+            sh[(threadIdx.x >> 5) * COLS + (me + S::TEAM * i) * S::VEC + k] = d[i * S::VEC + k];
         }
       }
       __syncthreads();
       for (int c = threadIdx.x; c < W; c += S::THREADS) {
         float s = first ? 0.f : out[c];
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) s += sh[w * S::COLS + c];
+        for (int w = 0; w < WARPS; ++w) s += sh[w * COLS + c];
         out[c] = s;
       }
     }
@@ -448,93 +516,75 @@ __device__ __forceinline__ void flush_cols(float (&dw)[S::N], float (&db)[S::N],
 
 constexpr int kChain = 128;   // rows that a thread adds up in fp32 before its sums join the partial rows
 
-// part NULL: dx alone; dx NULL: the column sums alone.
-template <class S>
-__global__ void __launch_bounds__(S::THREADS)
+// The statistics of the row after next, loaded ahead.
+struct Stats {
+  float mean, rstd;
+  __device__ __forceinline__ void load(const float* mean_in, const float* rstd_in, int64_t row, int64_t rows) {
+    mean = row < rows ? __ldg(mean_in + row) : 0.f;
+    rstd = row < rows ? __ldg(rstd_in + row) : 0.f;
+  }
+};
+
+// part NULL: dx alone; dx NULL: the column sums alone.  Beyond a row's end x is taken for the mean and g for 0.
+template <class S, bool SILU>
+__global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS)
 k_row_bwd(const typename S::T* __restrict__ x, int64_t ldx, const typename S::T* __restrict__ g, int64_t ldg, Norm n,
           const float* __restrict__ mean_in, const float* __restrict__ rstd_in, int64_t rows,
           typename S::T* __restrict__ dx, float* __restrict__ part) {
-  using P = Pack<typename S::T, S::VEC>;
-  __shared__ float sh[S::TEAM > 32 ? 2 * 5 * (S::TEAM / 32) : (S::THREADS / 32) * S::COLS];
+  using Raw = typename S::P::Raw;
+  __shared__ float sh[S::TEAM > 32 ? S::SCRATCH : S::THREADS / 32 * S::TEAM * S::N];
   int turn = 0;
-  const int me = threadIdx.x % S::TEAM, team = threadIdx.x / S::TEAM, W = (int)n.W;
+  const int me = threadIdx.x % S::TEAM, W = (int)n.W;
+  const int64_t step = gridDim.x * (int64_t)S::TEAMS;
   const float inv = 1.f / W;
-  float dw[S::N], db[S::N];
+  alignas(8) float dw[S::N], db[S::N];
 #pragma unroll
   for (int k = 0; k < S::N; ++k) dw[k] = db[k] = 0.f;
   int held = 0;
   bool first = true;
   if (part) part += blockIdx.x * (int64_t)(2 * W);
-  for (int64_t base = blockIdx.x * (int64_t)(S::TEAMS * S::RB); base < rows;
-       base += gridDim.x * (int64_t)(S::TEAMS * S::RB)) {
-    float xh[S::RB][S::N], h[S::RB][S::N], rstd[S::RB];
-    int64_t row[S::RB];
+  int64_t row = blockIdx.x * (int64_t)S::TEAMS + threadIdx.x / S::TEAM;
+  Rows<S, 2> operands{{x, g}, {ldx, ldg}, rows, step, W};
+  operands.load(row);
+  Stats next;
+  next.load(mean_in, rstd_in, row, rows);
+  for (int64_t base = blockIdx.x * (int64_t)S::TEAMS; base < rows; base += step, row += step) {
+    alignas(8) float v[2][S::N], ga[S::N], be[S::N];
+    operands.take(row, v);
+    const Stats st = next;
+    next.load(mean_in, rstd_in, row + step, rows);
+    columns<S>(n.gamma, W, 0.f, ga);      // beyond the row's end g is 0: so are its a and h
+    if (SILU) columns<S>(n.beta, W, 0.f, be);
+    if (!n.gamma) {
 #pragma unroll
-    for (int b = 0; b < S::RB; ++b) {
-      row[b] = base + b * S::TEAMS + team;
+      for (int k = 0; k < S::N; ++k) ga[k] = 1.f;
+    }
+    float2 s1 = f2(0.f), s2 = f2(0.f);
+#pragma unroll
+    for (int e = 0; e < S::N / 2; ++e) {
+      float2 &xh = E2A_PAIR(v[0], e), &h = E2A_PAIR(v[1], e);
+      xh = f2_mul(f2_add(xh, f2(-st.mean)), f2(st.rstd));
+      if (SILU) h = f2_mul(h, derivatives<SILU, false>(f2_fma(xh, E2A_PAIR(ga, e), E2A_PAIR(be, e))).d1);
+      E2A_PAIR(dw, e) = f2_fma(h, xh, E2A_PAIR(dw, e));
+      E2A_PAIR(db, e) = f2_add(h, E2A_PAIR(db, e));
+      h = f2_mul(h, E2A_PAIR(ga, e));
+      s1 = f2_add(s1, h);
+      s2 = f2_fma(h, xh, s2);
+    }
+    if (dx) {
+      float sums[2] = {s1.x + s1.y, s2.x + s2.y};
+      team_sum<S::TEAM>(sums, sh, turn);
+      const float2 m1 = f2(-sums[0] * inv * st.rstd), m2 = f2(-sums[1] * inv * st.rstd);
+#pragma unroll
+      for (int e = 0; e < S::N / 2; ++e)
+        E2A_PAIR(v[1], e) = f2_fma(E2A_PAIR(v[1], e), f2(st.rstd), f2_fma(E2A_PAIR(v[0], e), m2, m1));
 #pragma unroll
       for (int i = 0; i < S::V; ++i) {
         const int c = (me + S::TEAM * i) * S::VEC;
-        if (row[b] < rows && c < W) {
-          P::load(x + row[b] * ldx + c, xh[b] + i * S::VEC);
-          P::load(g + row[b] * ldg + c, h[b] + i * S::VEC);
-        } else {
-#pragma unroll
-          for (int k = 0; k < S::VEC; ++k) xh[b][i * S::VEC + k] = h[b][i * S::VEC + k] = 0.f;
-        }
+        if (row < rows && c < W) *reinterpret_cast<Raw*>(dx + row * W + c) = S::P::narrow(v[1] + i * S::VEC);
       }
     }
-    float sums[2 * S::RB];
-#pragma unroll
-    for (int b = 0; b < S::RB; ++b) {
-      const float mean = row[b] < rows ? mean_in[row[b]] : 0.f;
-      rstd[b] = row[b] < rows ? rstd_in[row[b]] : 0.f;
-      sums[2 * b] = sums[2 * b + 1] = 0.f;
-#pragma unroll
-      for (int k = 0; k < S::N; ++k) xh[b][k] = (xh[b][k] - mean) * rstd[b];
-    }
-#pragma unroll
-    for (int i = 0; i < S::V; ++i) {
-      const int c = (me + S::TEAM * i) * S::VEC;
-      if (c < W) {
-        float ga[S::VEC], be[S::VEC];
-        load_affine<S::VEC>(n.gamma, c, 1.f, ga);
-        load_affine<S::VEC>(n.beta, c, 0.f, be);
-#pragma unroll
-        for (int b = 0; b < S::RB; ++b) {
-#pragma unroll
-          for (int k = 0; k < S::VEC; ++k) {
-            const int e = i * S::VEC + k;
-            const float a = h[b][e] * activation(xh[b][e] * ga[k] + be[k], n.silu).d1;
-            dw[e] += a * xh[b][e];
-            db[e] += a;
-            h[b][e] = a * ga[k];
-            sums[2 * b] += h[b][e];
-            sums[2 * b + 1] += h[b][e] * xh[b][e];
-          }
-        }
-      }
-    }
-    if (dx) {
-      team_sum<S::TEAM>(sums, sh, turn);
-#pragma unroll
-      for (int b = 0; b < S::RB; ++b) {
-        const float m1 = sums[2 * b] * inv, m2 = sums[2 * b + 1] * inv;
-#pragma unroll
-        for (int i = 0; i < S::V; ++i) {
-          const int c = (me + S::TEAM * i) * S::VEC;
-          float o[S::VEC];
-#pragma unroll
-          for (int k = 0; k < S::VEC; ++k) {
-            const int e = i * S::VEC + k;
-            o[k] = rstd[b] * (h[b][e] - m1 - xh[b][e] * m2);
-          }
-          if (row[b] < rows && c < W) P::store(dx + row[b] * W + c, o);
-        }
-      }
-    }
-    held += S::RB;
-    if (part && held >= kChain) {
+    if (part && ++held == kChain) {
       flush_cols<S>(dw, db, part, W, first, sh);
       first = false;
       held = 0;
@@ -543,107 +593,126 @@ k_row_bwd(const typename S::T* __restrict__ x, int64_t ldx, const typename S::T*
   if (part && (held || first)) flush_cols<S>(dw, db, part, W, first, sh);
 }
 
-template <class S, bool PQ>
-__global__ void __launch_bounds__(S::THREADS)
+// Second order.  With B = r act', C = r g act'' w and d = u - <u> - xh c (t = r d):  dg = B w d (+ act' (p xh + q)),
+// e = C d,  dw = sum g B d + e xh,  k = w (e - c g B) - r <h xh> u; p and q join v = w t + p xh + q where they are.
+template <class S, bool SILU, bool PQ>
+__global__ void __launch_bounds__(S::THREADS, (S::N > 8 && S::THREADS <= 256 ? 256 : 512) / S::THREADS)
 k_row_bwd2(const typename S::T* __restrict__ x, int64_t ldx, const typename S::T* __restrict__ g, int64_t ldg,
            const typename S::T* __restrict__ u, int64_t ldu, Norm n, const float* __restrict__ mean_in,
            const float* __restrict__ rstd_in, int64_t rows, typename S::T* __restrict__ dg,
            typename S::T* __restrict__ dx, float* __restrict__ part) {
-  using P = Pack<typename S::T, S::VEC>;
-  __shared__ float sh[S::TEAM > 32 ? 2 * 5 * (S::TEAM / 32) : (S::THREADS / 32) * S::COLS];
+  using Raw = typename S::P::Raw;
+  __shared__ float sh[S::TEAM > 32 ? S::SCRATCH : S::THREADS / 32 * S::TEAM * S::N];
   int turn = 0;
-  const int me = threadIdx.x % S::TEAM, team = threadIdx.x / S::TEAM, W = (int)n.W;
+  const int me = threadIdx.x % S::TEAM, W = (int)n.W;
+  const int64_t step = gridDim.x * (int64_t)S::TEAMS;
   const float inv = 1.f / W;
-  float dw[S::N], db[S::N];
+  alignas(8) float dw[S::N], db[S::N];
 #pragma unroll
   for (int k = 0; k < S::N; ++k) dw[k] = db[k] = 0.f;
   int held = 0;
   bool first = true;
   if (part) part += blockIdx.x * (int64_t)(2 * W);
-  for (int64_t base = blockIdx.x * (int64_t)S::TEAMS; base < rows; base += gridDim.x * (int64_t)S::TEAMS) {
-    const int64_t row = base + team;
+  int64_t row = blockIdx.x * (int64_t)S::TEAMS + threadIdx.x / S::TEAM;
+  Rows<S, 3> operands{{x, g, u}, {ldx, ldg, ldu}, rows, step, W};
+  operands.load(row);
+  Stats next;
+  next.load(mean_in, rstd_in, row, rows);
+  for (int64_t base = blockIdx.x * (int64_t)S::TEAMS; base < rows; base += step, row += step) {
+    alignas(8) float v[3][S::N], ga[S::N], be[S::N], B[S::N], C[S::N];
+    operands.take(row, v);
+    const Stats st = next;
+    next.load(mean_in, rstd_in, row + step, rows);
+    columns<S>(n.gamma, W, 1.f, ga);
+    if (SILU) columns<S>(n.beta, W, 0.f, be);
+    const float2 r = f2(st.rstd);
+    float2 s[5];      // u, u xh, r h, r h xh, r h u; beyond the row's end g and u are 0
+#pragma unroll
+    for (int i = 0; i < 5; ++i) s[i] = f2(0.f);
+#pragma unroll
+    for (int e = 0; e < S::N / 2; ++e) {
+      float2& xh = E2A_PAIR(v[0], e);
+      const float2 gv = E2A_PAIR(v[1], e), uv = E2A_PAIR(v[2], e), w = E2A_PAIR(ga, e);
+      xh = f2_mul(f2_add(xh, f2(-st.mean)), r);
+      const Act2 a = derivatives<SILU, true>(SILU ? f2_fma(xh, w, E2A_PAIR(be, e)) : xh);
+      E2A_PAIR(B, e) = SILU ? f2_mul(a.d1, r) : r;
+      E2A_PAIR(C, e) = SILU ? f2_mul(f2_mul(gv, a.d2), f2_mul(w, r)) : f2(0.f);
+      const float2 rh = f2_mul(f2_mul(gv, E2A_PAIR(B, e)), w);
+      s[0] = f2_add(s[0], uv);
+      s[1] = f2_fma(uv, xh, s[1]);
+      s[2] = f2_add(s[2], rh);
+      s[3] = f2_fma(rh, xh, s[3]);
+      s[4] = f2_fma(rh, uv, s[4]);
+    }
+    float s5[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) s5[i] = s[i].x + s[i].y;
+    team_sum<S::TEAM>(s5, sh, turn);
+    const float su = s5[0] * inv, sc = s5[1] * inv, m2 = s5[3] * inv;     // <u>, c, r <h xh>
+    const float ht = s5[4] * inv - s5[2] * inv * su - m2 * sc;            // <h t>
     const bool in = row < rows;
-    float xh[S::N], gv[S::N], uv[S::N];
+    float2 k1 = f2(0.f), k2 = f2(0.f);
+    alignas(8) float pc[S::N], qc[S::N];
+    if (PQ) {
+      columns<S>(n.p, W, 0.f, pc);
+      columns<S>(n.q, W, 0.f, qc);
+    }
+#pragma unroll
+    for (int e = 0; e < S::N / 2; ++e) {
+      const float2 xh = E2A_PAIR(v[0], e), w = E2A_PAIR(ga, e), gv = E2A_PAIR(v[1], e);
+      float2& uv = E2A_PAIR(v[2], e);
+      float2 d = f2_fma(xh, f2(-sc), f2_add(uv, f2(-su)));
+      const float2 gB = f2_mul(gv, E2A_PAIR(B, e));
+      float2 er = f2_mul(E2A_PAIR(C, e), d);
+      float2 out = f2_mul(f2_mul(E2A_PAIR(B, e), w), d);
+      float2 kk = f2_fma(gB, f2(-sc), er);
+      if (PQ) {      // v's other share o = p xh + q: act' o, e + g act'' o, k + act' g p
+        const float2 o = f2_fma(E2A_PAIR(pc, e), xh, E2A_PAIR(qc, e));
+        const Act2 a = derivatives<SILU, true>(SILU ? f2_fma(xh, w, E2A_PAIR(be, e)) : xh);
+        out = f2_fma(a.d1, o, out);
+        const float2 more = f2_mul(f2_mul(gv, a.d2), o);
+        kk = f2_add(kk, more);
+        er = f2_add(er, more);
+        kk = f2_mul(kk, w);
+        kk = f2_fma(f2_mul(gv, a.d1), E2A_PAIR(pc, e), kk);
+      } else {
+        kk = f2_mul(kk, w);
+      }
+      kk = f2_fma(uv, f2(-m2), kk);
+      E2A_PAIR(dw, e) = f2_fma(gB, d, E2A_PAIR(dw, e));
+      if (SILU) {
+        E2A_PAIR(dw, e) = f2_fma(er, xh, E2A_PAIR(dw, e));
+        E2A_PAIR(db, e) = f2_add(er, E2A_PAIR(db, e));
+      }
+      E2A_PAIR(v[1], e) = out;
+      uv = kk;
+    }
 #pragma unroll
     for (int i = 0; i < S::V; ++i) {
       const int c = (me + S::TEAM * i) * S::VEC;
-      if (in && c < W) {
-        P::load(x + row * ldx + c, xh + i * S::VEC);
-        P::load(g + row * ldg + c, gv + i * S::VEC);
-        P::load(u + row * ldu + c, uv + i * S::VEC);
+      if (c < W) {
+        if (in) *reinterpret_cast<Raw*>(dg + row * W + c) = S::P::narrow(v[1] + i * S::VEC);
       } else {
 #pragma unroll
-        for (int k = 0; k < S::VEC; ++k) xh[i * S::VEC + k] = gv[i * S::VEC + k] = uv[i * S::VEC + k] = 0.f;
+        for (int k = 0; k < S::VEC; ++k) v[2][i * S::VEC + k] = 0.f;
       }
     }
-    const float mean = in ? mean_in[row] : 0.f, rstd = in ? rstd_in[row] : 0.f;
-    float s5[5] = {0.f, 0.f, 0.f, 0.f, 0.f};    // u, u xh, h, h xh, h u
 #pragma unroll
-    for (int i = 0; i < S::V; ++i) {
-      const int c = (me + S::TEAM * i) * S::VEC;
-      if (c < W) {
-        float ga[S::VEC], be[S::VEC];
-        load_affine<S::VEC>(n.gamma, c, 1.f, ga);
-        load_affine<S::VEC>(n.beta, c, 0.f, be);
-#pragma unroll
-        for (int k = 0; k < S::VEC; ++k) {
-          const int e = i * S::VEC + k;
-          xh[e] = (xh[e] - mean) * rstd;
-          const float h = gv[e] * activation(xh[e] * ga[k] + be[k], n.silu).d1 * ga[k];
-          s5[0] += uv[e];
-          s5[1] += uv[e] * xh[e];
-          s5[2] += h;
-          s5[3] += h * xh[e];
-          s5[4] += h * uv[e];
-        }
-      }
+    for (int e = 0; e < S::N / 2; ++e) {
+      k1 = f2_add(k1, E2A_PAIR(v[2], e));
+      k2 = f2_fma(E2A_PAIR(v[2], e), E2A_PAIR(v[0], e), k2);
     }
-    team_sum<S::TEAM>(s5, sh, turn);
-    const float su = s5[0] * inv, sc = s5[1] * inv, m2 = s5[3] * inv;
-    const float ht = rstd * (s5[4] * inv - s5[2] * inv * su - m2 * sc);
-    float s2[2] = {0.f, 0.f};                   // k, k xh
-#pragma unroll
-    for (int i = 0; i < S::V; ++i) {
-      const int c = (me + S::TEAM * i) * S::VEC;
-      if (c < W) {
-        float ga[S::VEC], be[S::VEC], pc[S::VEC], qc[S::VEC], o[S::VEC];
-        load_affine<S::VEC>(n.gamma, c, 1.f, ga);
-        load_affine<S::VEC>(n.beta, c, 0.f, be);
-        if (PQ) {
-          load_affine<S::VEC>(n.p, c, 0.f, pc);
-          load_affine<S::VEC>(n.q, c, 0.f, qc);
-        }
-#pragma unroll
-        for (int k = 0; k < S::VEC; ++k) {
-          const int e = i * S::VEC + k;
-          const Act a = activation(xh[e] * ga[k] + be[k], n.silu);
-          const float t = rstd * (uv[e] - su - xh[e] * sc);
-          const float v = PQ ? ga[k] * t + pc[k] * xh[e] + qc[k] : ga[k] * t;
-          const float ag = gv[e] * a.d1, er = gv[e] * a.d2 * v;
-          o[k] = a.d1 * v;
-          dw[e] += ag * t + er * xh[e];
-          db[e] += er;
-          float kk = er * ga[k] - rstd * (uv[e] * m2 + ag * ga[k] * sc);
-          if (PQ) kk += ag * pc[k];
-          uv[e] = kk;
-          s2[0] += kk;
-          s2[1] += kk * xh[e];
-        }
-        if (in) P::store(dg + row * W + c, o);
-      }
-    }
+    float s2[2] = {k1.x + k1.y, k2.x + k2.y};
     team_sum<S::TEAM>(s2, sh, turn);
-    const float k1 = s2[0] * inv, k2 = s2[1] * inv + ht;
+    k1 = f2(-s2[0] * inv * st.rstd);
+    k2 = f2(-(s2[1] * inv + ht) * st.rstd);
+#pragma unroll
+    for (int e = 0; e < S::N / 2; ++e)
+      E2A_PAIR(v[2], e) = f2_fma(E2A_PAIR(v[2], e), r, f2_fma(E2A_PAIR(v[0], e), k2, k1));
 #pragma unroll
     for (int i = 0; i < S::V; ++i) {
       const int c = (me + S::TEAM * i) * S::VEC;
-      float o[S::VEC];
-#pragma unroll
-      for (int k = 0; k < S::VEC; ++k) {
-        const int e = i * S::VEC + k;
-        o[k] = rstd * (uv[e] - k1 - xh[e] * k2);
-      }
-      if (in && c < W) P::store(dx + row * W + c, o);
+      if (in && c < W) *reinterpret_cast<Raw*>(dx + row * W + c) = S::P::narrow(v[2] + i * S::VEC);
     }
     if (part && ++held == kChain) {
       flush_cols<S>(dw, db, part, W, first, sh);
@@ -690,29 +759,33 @@ bool vectors_fit(const Norm& n, const void* const* rows_of, const int64_t* ld, i
   return aligned16(n.gamma) && aligned16(n.beta) && aligned16(n.p) && aligned16(n.q);
 }
 
-// Calls f with the Shape for rows of W values: the smallest team that holds a row, 16 values a thread at most.
-template <typename T, typename F>
+// Calls f with the Shape for rows of W values: two vectors a thread while a warp holds the row so, then 16 values,
+// then WIDE in teams of a CTA, the smallest that holds a row.  640,210 x 128 fp32: 16 values a thread take the
+// backward from 161 to 190 us; 16,384 x 4,096 bf16: 32 take the forward from 62 to 49 us, the backward from 81 to
+// 99 us (registers).
+template <typename T, int WIDE, typename F>
 int by_shape(int64_t W, bool vec, F f) {
-  constexpr int VEC = 16 / sizeof(T), V4 = 16 / VEC;
+  constexpr int VEC = 16 / sizeof(T), V16 = 16 / VEC, VW = WIDE / VEC;
   if (vec) {
-    if (W <= 4 * VEC) return f(Shape<T, VEC, 1, 4, V4>{});
-    if (W <= 8 * VEC) return f(Shape<T, VEC, 1, 8, V4>{});
-    if (W <= 16 * VEC) return f(Shape<T, VEC, 1, 16, V4>{});
-    if (W <= 32 * VEC) return f(Shape<T, VEC, 1, 32, V4>{});
-    if (VEC == 4 && W <= 256) return f(Shape<T, VEC, 2, 32, V4 / 2>{});
-    if (W <= 512) return f(Shape<T, VEC, V4, 32, 1>{});
-    if (W <= 1024) return f(Shape<T, VEC, V4, 64, 1>{});
-    if (W <= 2048) return f(Shape<T, VEC, V4, 128, 1>{});
-    if (W <= 4096) return f(Shape<T, VEC, V4, 256, 1>{});
-    return f(Shape<T, VEC, V4, 512, 1>{});
+    if (W <= 4 * VEC) return f(Shape<T, VEC, 1, 4>{});
+    if (W <= 8 * VEC) return f(Shape<T, VEC, 2, 4>{});
+    if (W <= 16 * VEC) return f(Shape<T, VEC, 2, 8>{});
+    if (W <= 32 * VEC) return f(Shape<T, VEC, 2, 16>{});
+    if (W <= 64 * VEC) return f(Shape<T, VEC, 2, 32>{});
+    if (W <= 512) return f(Shape<T, VEC, V16, 32>{});
+    if (W <= 32 * WIDE) return f(Shape<T, VEC, VW, 32>{});
+    if (W <= 64 * WIDE) return f(Shape<T, VEC, VW, 64>{});
+    if (W <= 128 * WIDE) return f(Shape<T, VEC, VW, 128>{});
+    if (W <= 256 * WIDE) return f(Shape<T, VEC, VW, 256>{});
+    return f(Shape<T, VEC, V16, 512>{});
   }
-  if (W <= 32) return f(Shape<T, 1, 4, 8, 2>{});
-  if (W <= 128) return f(Shape<T, 1, 4, 32, 2>{});
-  if (W <= 512) return f(Shape<T, 1, 16, 32, 1>{});
-  if (W <= 1024) return f(Shape<T, 1, 16, 64, 1>{});
-  if (W <= 2048) return f(Shape<T, 1, 16, 128, 1>{});
-  if (W <= 4096) return f(Shape<T, 1, 16, 256, 1>{});
-  return f(Shape<T, 1, 16, 512, 1>{});
+  if (W <= 32) return f(Shape<T, 1, 4, 8>{});
+  if (W <= 128) return f(Shape<T, 1, 4, 32>{});
+  if (W <= 512) return f(Shape<T, 1, 16, 32>{});
+  if (W <= 1024) return f(Shape<T, 1, 16, 64>{});
+  if (W <= 2048) return f(Shape<T, 1, 16, 128>{});
+  if (W <= 4096) return f(Shape<T, 1, 16, 256>{});
+  return f(Shape<T, 1, 16, 512>{});
 }
 
 // Partial rows of column sums, one per CTA of a row kernel.
@@ -723,17 +796,23 @@ int64_t most_parts(int64_t rows, int64_t W) {
 
 // CTAs of a row kernel: as many as the device holds at once, never more than there are batches of rows.
 template <auto Kernel, class S>
-int row_grid(int64_t rows, int64_t W, int rb) {
-  static const int resident = [] {
-    int dev = 0, sms = 148, per = 1;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, Kernel, S::THREADS, 0);
-    return sms * (per > 0 ? per : 1);
-  }();
-  const int64_t batches = (rows + S::TEAMS * rb - 1) / (S::TEAMS * rb), most = most_parts(rows, W);
-  int64_t g = batches < resident ? batches : resident;
-  return (int)(g < most ? g : most);
+int row_grid(int64_t rows, int64_t W, int* grid) {
+  static std::atomic<int> resident_on[64];
+  int dev = 0;
+  E2A_CUDA(cudaGetDevice(&dev));
+  std::atomic<int>& known = resident_on[dev & 63];
+  int resident = dev < 64 ? known.load(std::memory_order_relaxed) : 0;
+  if (resident == 0) {
+    int sms = 0, per = 0;
+    E2A_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    E2A_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, Kernel, S::THREADS, 0));
+    resident = sms * (per > 0 ? per : 1);
+    known.store(resident, std::memory_order_relaxed);
+  }
+  const int64_t batches = (rows + S::TEAMS - 1) / S::TEAMS, most = most_parts(rows, W);
+  const int64_t g = batches < resident ? batches : resident;
+  *grid = (int)(g < most ? g : most);
+  return E2A_OK;
 }
 
 int sum_parts(const float* part, int n_part, int64_t W, float* dw, float* db, cudaStream_t st) {
@@ -784,6 +863,11 @@ int by_type(int dtype, F f) {
   }
 }
 
+template <typename F>
+int by_flag(bool flag, F f) {
+  return flag ? f(std::true_type{}) : f(std::false_type{});
+}
+
 int zero_cols(float* dw, float* db, int64_t W, cudaStream_t st) {
   if (dw) E2A_CUDA(cudaMemsetAsync(dw, 0, W * sizeof(float), st));
   if (db) E2A_CUDA(cudaMemsetAsync(db, 0, W * sizeof(float), st));
@@ -805,12 +889,16 @@ int e2a_layer_norm_fwd(const void* x, int64_t ldx, int dtype, const float* gamma
     if (W <= kMaxTeamWidth) {
       const void* of[] = {x, y};
       const int64_t ld[] = {ldx, W};
-      return by_shape<T>(W, vectors_fit<T>(n, of, ld, 2), [&](auto shape) -> int {
+      return by_shape<T, 32>(W, vectors_fit<T>(n, of, ld, 2), [&](auto shape) -> int {
         using S = decltype(shape);
-        const int grid = row_grid<&k_row_fwd<S>, S>(rows, W, S::RB);
-        k_row_fwd<S><<<grid, S::THREADS, 0, (cudaStream_t)stream>>>((const T*)x, ldx, n, rows, eps, (T*)y, mean, rstd);
-        E2A_CHECK_LAUNCH();
-        return E2A_OK;
+        return by_flag(n.silu, [&](auto silu) -> int {
+          constexpr auto kernel = &k_row_fwd<S, silu.value>;
+          int grid = 0;
+          if (const int rc = row_grid<kernel, S>(rows, W, &grid)) return rc;
+          kernel<<<grid, S::THREADS, 0, (cudaStream_t)stream>>>((const T*)x, ldx, n, rows, eps, (T*)y, mean, rstd);
+          E2A_CHECK_LAUNCH();
+          return E2A_OK;
+        });
       });
     }
     k_ln_fwd<T><<<grid_rows(rows), kThreads, 0, (cudaStream_t)stream>>>((const T*)x, ldx, n, rows, eps, (T*)y, mean,
@@ -839,14 +927,17 @@ int e2a_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy,
     if (W <= kMaxTeamWidth) {
       const void* of[] = {x, dy, dx};
       const int64_t ld[] = {ldx, lddy, W};
-      return by_shape<T>(W, vectors_fit<T>(n, of, ld, 3), [&](auto shape) -> int {
+      return by_shape<T, 16>(W, vectors_fit<T>(n, of, ld, 3), [&](auto shape) -> int {
         using S = decltype(shape);
         float* part = dgamma || dbeta ? (float*)workspace : nullptr;
-        const int grid = row_grid<&k_row_bwd<S>, S>(rows, W, S::RB);
-        k_row_bwd<S><<<grid, S::THREADS, 0, st>>>((const T*)x, ldx, (const T*)dy, lddy, n, mean, rstd, rows, (T*)dx,
-                                                  part);
-        E2A_CHECK_LAUNCH();
-        return part ? sum_parts(part, grid, W, dgamma, dbeta, st) : E2A_OK;
+        return by_flag(n.silu, [&](auto silu) -> int {
+          constexpr auto kernel = &k_row_bwd<S, silu.value>;
+          int grid = 0;
+          if (const int rc = row_grid<kernel, S>(rows, W, &grid)) return rc;
+          kernel<<<grid, S::THREADS, 0, st>>>((const T*)x, ldx, (const T*)dy, lddy, n, mean, rstd, rows, (T*)dx, part);
+          E2A_CHECK_LAUNCH();
+          return part ? sum_parts(part, grid, W, dgamma, dbeta, st) : E2A_OK;
+        });
       });
     }
     if (dx) {
@@ -883,16 +974,20 @@ int e2a_layer_norm_bwd2(const void* x, int64_t ldx, const void* dy, int64_t lddy
     if (W <= kMaxTeamWidth) {
       const void* of[] = {x, dy, u, d_dy, dx};
       const int64_t ld[] = {ldx, lddy, ldu, W, W};
-      return by_shape<T>(W, vectors_fit<T>(n, of, ld, 5), [&](auto shape) -> int {
+      return by_shape<T, 16>(W, vectors_fit<T>(n, of, ld, 5), [&](auto shape) -> int {
         using S = decltype(shape);
         float* sums = dgamma || dbeta ? (float*)part : nullptr;
-        auto* kernel = p || q ? k_row_bwd2<S, true> : k_row_bwd2<S, false>;
-        const int grid = p || q ? row_grid<&k_row_bwd2<S, true>, S>(rows, W, 1)
-                                : row_grid<&k_row_bwd2<S, false>, S>(rows, W, 1);
-        kernel<<<grid, S::THREADS, 0, st>>>((const T*)x, ldx, (const T*)dy, lddy, (const T*)u, ldu, n, mean, rstd, rows,
-                                            (T*)d_dy, (T*)dx, sums);
-        E2A_CHECK_LAUNCH();
-        return sums ? sum_parts(sums, grid, W, dgamma, dbeta, st) : E2A_OK;
+        return by_flag(n.silu, [&](auto silu) -> int {
+          return by_flag(p || q, [&](auto pq) -> int {
+            constexpr auto kernel = &k_row_bwd2<S, silu.value, pq.value>;
+            int grid = 0;
+            if (const int rc = row_grid<kernel, S>(rows, W, &grid)) return rc;
+            kernel<<<grid, S::THREADS, 0, st>>>((const T*)x, ldx, (const T*)dy, lddy, (const T*)u, ldu, n, mean, rstd,
+                                                    rows, (T*)d_dy, (T*)dx, sums);
+            E2A_CHECK_LAUNCH();
+            return sums ? sum_parts(sums, grid, W, dgamma, dbeta, st) : E2A_OK;
+          });
+        });
       });
     }
     k_ln_bwd2<T><<<grid_rows(rows), kThreads, 0, st>>>((const T*)x, ldx, (const T*)dy, lddy, (const T*)u, ldu, n, mean,
