@@ -99,7 +99,7 @@ SIGNATURES = {
 }
 
 _lib = None
-_tensors = None
+_torch = None
 
 
 E2A_ERR_UNSUPPORTED = 4   # status of an entry point that does not take the given operands (include/e2a.h)
@@ -126,19 +126,32 @@ def load():
     return lib
 
 
-def load_tensors():
-    """``libe2a_tensors.so``, which reads a list of tensors in one call (with the interpreter's lock held)."""
-    global _tensors
-    if _tensors is None:
-        path = os.path.join(_HERE, "libe2a_tensors.so")
+# what libe2a_torch.so calls of libe2a.so, in its order
+_TORCH_ENTRIES = ("e2a_layer_norm_fwd", "e2a_layer_norm_bwd_workspace_bytes", "e2a_layer_norm_bwd",
+                  "e2a_layer_norm_bwd2_workspace_bytes", "e2a_layer_norm_bwd2", "e2a_status_string",
+                  "e2a_last_cuda_error")
+
+
+def load_torch():
+    """``libe2a_torch.so``, host code against PyTorch's C++ interface (called with the interpreter's lock held);
+    its kernels are those of :func:`load`'s library."""
+    global _torch
+    if _torch is None:
+        path = os.path.join(_HERE, "libe2a_torch.so")
         if not os.path.exists(path):
-            raise E2AError(f"libe2a_tensors.so not found at {path}: build it with `python __graft_entry__.py` "
+            raise E2AError(f"libe2a_torch.so not found at {path}: build it with `python __graft_entry__.py` "
                            "or `make -C ubio_molfm_b200/csrc`")
-        lib = ctypes.PyDLL(path)
+        lib, kernels = ctypes.PyDLL(path), load()
         lib.e2a_tensor_table.restype = I32
         lib.e2a_tensor_table.argtypes = [ctypes.py_object, I64, P, P, P, P, P]
-        _tensors = lib
-    return _tensors
+        lib.e2a_layer_norm.restype = ctypes.py_object
+        lib.e2a_layer_norm.argtypes = [ctypes.py_object, ctypes.py_object, ctypes.py_object, F64, I32]
+        lib.e2a_torch_bind.restype = None
+        lib.e2a_torch_bind.argtypes = [P]
+        lib.e2a_torch_bind((P * len(_TORCH_ENTRIES))(*(ctypes.cast(getattr(kernels, n), P).value
+                                                       for n in _TORCH_ENTRIES)))
+        _torch = lib
+    return _torch
 
 
 def launch_count() -> int:

@@ -32,11 +32,11 @@ def _pointers(tensors):
 
 def _table(tensors, with_grads=False):
     """``(addresses, sizes, addresses of the gradients or None, type code, device index)`` of a list of tensors
-    in one call, or None where they are not all alike (see ``csrc/e2a_tensors.cpp``)."""
+    in one call, or None where they are not all alike (see ``csrc/e2a_torch.cpp``)."""
     n = len(tensors)
     at, numel, two = array("Q", (0,)) * n, array("q", (0,)) * n, array("i", (0, 0))
     grads = array("Q", (0,)) * n if with_grads else None
-    if _lib.load_tensors().e2a_tensor_table(tensors, n, _address(at), _address(numel),
+    if _lib.load_torch().e2a_tensor_table(tensors, n, _address(at), _address(numel),
                                             _address(grads) if with_grads else None, _address(two),
                                             _address(two) + 4):
         return None
