@@ -149,7 +149,7 @@ class E2AttentionArbOrder_sparse(nn.Module):
             h = attn_weight.linear(w[:, :nb], lin0.bias, cw)
         else:
             h = lin(attn_weight, w[:, :nb], lin0.bias, cw)
-        h = run_mlp(list(net)[1:], h, cw, first_tables=(t_tab, z_q, s_tab, z_k))
+        h = run_mlp(list(net)[1:], h, cw, first_tables=(t_tab, z_q, s_tab, z_k), fused_norm=self.fc_easy.fused_norm)
         return h  # [E, 2H]: gate = [:, :H], inputhead = [:, H:]
 
     def _edge_chunks(self, bd, n_rows):

@@ -246,13 +246,11 @@ void check_affine(const Tensor& t, const Tensor& x, const char* name) {
 
 extern "C" {
 
-// Addresses and numbers of elements of `tensors` (a list of n).  With `grads` also those of each one's .grad.
-// Returns 0 with *type and *device where all are strided, contiguous CUDA tensors of one supported type on one
-// device (and every gradient exists, as long as its parameter); 1 where not, or on any error: the caller then
-// looks at them one by one and says what is wrong.
+// Addresses and numbers of elements of `tensors` (a list of n > 0).  Returns 0 with *type and *device where all are
+// strided, contiguous CUDA tensors of one supported type on one device; 1 where not, or on any error: the caller
+// then looks at them one by one and says what is wrong.
 __attribute__((visibility("default"))) int e2a_tensor_table(PyObject* tensors, int64_t n, uint64_t* address,
-                                                            int64_t* numel, uint64_t* grads, int32_t* type,
-                                                            int32_t* device) {
+                                                            int64_t* numel, int32_t* type, int32_t* device) {
   try {
     if (!PyList_CheckExact(tensors) || PyList_GET_SIZE(tensors) != n || n == 0) return 1;
     Common all;
@@ -263,14 +261,46 @@ __attribute__((visibility("default"))) int e2a_tensor_table(PyObject* tensors, i
       if (!all.take(t)) return 1;
       address[j] = reinterpret_cast<uint64_t>(t.data_ptr());
       numel[j] = t.numel();
-      if (grads) {
-        const Tensor& g = t.grad();
-        if (!g.defined() || !all.take(g) || g.numel() != numel[j]) return 1;
-        grads[j] = reinterpret_cast<uint64_t>(g.data_ptr());
-      }
     }
     *type = all.type;
     *device = all.device;
+    return 0;
+  } catch (...) {
+    return 1;
+  }
+}
+
+// The optimiser's table of a list of n parameters: for the *count of them that have a gradient, in order, the
+// addresses of both, their number of elements (that of held_numel, or 1 is returned), their held_offset and their
+// place in the list; counts a new version of each, since the kernels write behind autograd's back.  Returns as
+// above, with *count 0 and no type where no parameter has a gradient.
+__attribute__((visibility("default"))) int e2a_step_table(PyObject* params, int64_t n, const int64_t* held_numel,
+                                                          const int64_t* held_offset, uint64_t* address,
+                                                          uint64_t* grads, int64_t* numel, int64_t* offset,
+                                                          int32_t* slot, int32_t* type, int32_t* device,
+                                                          int32_t* count) {
+  try {
+    if (!PyList_CheckExact(params) || PyList_GET_SIZE(params) != n) return 1;
+    Common all;
+    int32_t k = 0;
+    for (int64_t j = 0; j < n; ++j) {
+      PyObject* o = PyList_GET_ITEM(params, j);
+      if (!THPVariable_Check(o)) return 1;
+      const Tensor& t = THPVariable_Unpack(o);
+      const Tensor& g = t.grad();
+      if (!g.defined()) continue;
+      if (!all.take(t) || !all.take(g) || t.numel() != held_numel[j] || g.numel() != held_numel[j]) return 1;
+      address[k] = reinterpret_cast<uint64_t>(t.data_ptr());
+      grads[k] = reinterpret_cast<uint64_t>(g.data_ptr());
+      numel[k] = held_numel[j];
+      offset[k] = held_offset[j];
+      slot[k++] = (int32_t)j;
+    }
+    for (int32_t i = 0; i < k; ++i)
+      torch::autograd::impl::bump_version(THPVariable_Unpack(PyList_GET_ITEM(params, slot[i])));
+    *type = all.type;
+    *device = all.device;
+    *count = k;
     return 0;
   } catch (...) {
     return 1;

@@ -21,6 +21,7 @@ import contextlib
 import numpy as np
 import torch
 
+from . import _lib
 from . import linear
 from .model import E2FormerPotential
 
@@ -153,6 +154,31 @@ class E2FormerModelInterface:
         if need_force:
             out["pred_forces"] = forces
         return out
+
+    def train_step(self, model_input, energy, forces, optimizer, energy_weight=1.0, force_weight=1.0):
+        """One step of force-loss training on a collated batch: the model in training mode, ``loss =
+        energy_weight mean_B ((E - energy) / atoms)^2 + force_weight mean_atoms |F - forces|^2`` (``energy`` [B],
+        ``forces`` [B,L,3], read on the real atoms), its backward through the forces' graph, and
+        ``optimizer.step()`` (e.g. :class:`~ubio_molfm_b200.optim.AdamW`, which also clips).  Returns the loss
+        (0-dim, on the device); the model is back in the mode it was in."""
+        mode = self.model.training
+        mask = model_input["atom_masks"].to(self.device).bool()
+        counts = mask.sum(-1).clamp(min=1)
+        self.model.train()
+        try:
+            out = self.predict(model_input)
+            de = (out["pred_energy"] - torch.as_tensor(energy, device=self.device).reshape(-1)) / counts
+            df = (out["pred_forces"] - torch.as_tensor(forces, device=self.device))[mask]
+            loss = energy_weight * de.square().mean() + force_weight * df.square().sum(-1).mean()
+            optimizer.zero_grad()
+            with projection_precision("tf32" if self.use_tf32 else "fp32"):
+                loss.backward()
+            if self.model.check_device_status:
+                _lib.raise_on_device_status(self.device)      # before the gradients are used
+            optimizer.step()
+        finally:
+            self.model.train(mode)
+        return loss.detach()
 
     def __call__(self, *args, **kwargs):
         return self.predict(*args, **kwargs)

@@ -231,7 +231,7 @@ class EdgeDegreeEmbeddingNetwork_higherorder(nn.Module):
                     h = edge_scalars.linear(w[:, :nb], lin0.bias, cw)
                 else:
                     h = lin(edge_scalars, w[:, :nb], lin0.bias, cw)
-                h = run_mlp(layers[1:], h, cw, first_tables=(t_tab, z_q, s_tab, z_k))
+                h = run_mlp(layers[1:], h, cw, first_tables=(t_tab, z_q, s_tab, z_k), fused_norm=prof.fused_norm)
             else:
                 h = prof(edge_scalars.materialize() if isinstance(edge_scalars, RbfSpec) else edge_scalars)
             # the envelope scales each edge's product: applied to the [E, 2l+1] harmonics rather than the
@@ -412,7 +412,8 @@ class E2FormerPotential(nn.Module):
     ``(energy [B], forces [N,3])``.  Periodic systems are one per call; non-periodic molecules may be
     batched (``batch`` sorted, systems do not see each other)."""
 
-    def __init__(self, memory_saving="auto", use_faiss=False, edge_chunk=None, **backbone_kwargs):
+    def __init__(self, memory_saving="auto", use_faiss=False, edge_chunk=None, fused_layer_norm=False,
+                 **backbone_kwargs):
         super().__init__()
         # use_faiss: expanded nodes in the order of the reference's FAISS neighbour path
         # (distributed_cell_expand, one image cell per direction) instead of CellExpander's; the edges
@@ -436,6 +437,12 @@ class E2FormerPotential(nn.Module):
         self.memory_saving = memory_saving
         self.edge_chunk = edge_chunk
         self._set_memory_mode(memory_saving is True, memory_saving is not True, edge_chunk)
+        # fused_layer_norm: in training mode every LayerNorm of the radial and scalar MLPs and the SiLU after
+        # it run as one kernel (norm.layer_norm) forward, backward and second order, instead of PyTorch's
+        # (the same to fp32 rounding; eval mode has its own fused kernel and is not changed)
+        for m in self.modules():
+            if hasattr(m, "fused_norm"):
+                m.fused_norm = bool(fused_layer_norm)
 
     def _set_memory_mode(self, recompute, keep_logits, edge_chunk=None):
         for blk in self.decoder.blocks:

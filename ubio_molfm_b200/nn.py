@@ -13,6 +13,7 @@ import torch
 from torch import nn
 
 from . import linear as tc
+from . import norm
 from .cg import so2_first_order_tables
 
 
@@ -111,6 +112,7 @@ class SO3_Linear2Scalar_e2former(nn.Module):
         self.register_buffer("expand_index", expand_index)
         self.final_linear = nn.Sequential(
             nn.Linear(hidden * (lmax + 1), hidden), nn.LayerNorm(hidden), nn.SiLU(), nn.Linear(hidden, out_features))
+        self.fused_norm = False      # training: the LayerNorm and SiLU of final_linear as one kernel
         # inference memory mode: form the per-degree projections again in the backward instead of
         # keeping them (4 x hidden floats per irreps row)
         self.recompute_pair_product = False
@@ -139,7 +141,12 @@ class SO3_Linear2Scalar_e2former(nn.Module):
             if l == 0:
                 o1 = o1 + self.bias.reshape(1, 1, -1)
             parts.append((o1 * o2).sum(dim=1))
-        out = self.final_linear(torch.cat(parts, dim=-1))
+        h = torch.cat(parts, dim=-1)
+        if self.fused_norm and h.is_cuda:
+            fl = self.final_linear
+            out = fl[3](norm.layer_norm(fl[0](h), fl[1].weight, fl[1].bias, fl[1].eps, "silu"))
+        else:
+            out = self.final_linear(h)
         return out.reshape(*shape, self.out_features)
 
 
@@ -159,14 +166,16 @@ class RadialProfile(nn.Module):
                 mods.append(nn.LayerNorm(ch_list[i]))
             mods.append(nn.SiLU())
         self.net = nn.Sequential(*mods)
+        self.fused_norm = False      # training: each LayerNorm and its SiLU as one kernel
 
     def forward(self, f_in):
-        return run_mlp(list(self.net), f_in, not self.training)
+        return run_mlp(list(self.net), f_in, not self.training, fused_norm=self.fused_norm)
 
 
-def run_mlp(layers, h, const_weights, first_tables=None):
+def run_mlp(layers, h, const_weights, first_tables=None, fused_norm=False):
     """Linear / LayerNorm / SiLU stack; on CUDA in eval mode each LayerNorm+SiLU pair is one fused kernel
-    (``first_tables`` are added to the first Linear's output inside that fused kernel)."""
+    (``first_tables`` are added to the first Linear's output inside that fused kernel).  In training
+    ``fused_norm`` makes each pair one kernel too, with the parameters' gradients to second order."""
     i = 0
     pending = first_tables
     while i < len(layers):
@@ -185,6 +194,11 @@ def run_mlp(layers, h, const_weights, first_tables=None):
                 T, zt, S, zs = pending
                 h = h + T[zt] + S[zs]
                 pending = None
+            if (fused_norm and h.is_cuda and not const_weights and isinstance(layer, nn.LayerNorm)
+                    and i + 1 < len(layers) and isinstance(layers[i + 1], nn.SiLU)):
+                h = norm.layer_norm(h, layer.weight, layer.bias, layer.eps, "silu")
+                i += 2
+                continue
             h = layer(h)
             i += 1
     return h

@@ -30,17 +30,18 @@ def _pointers(tensors):
     return array("Q", map(torch.Tensor.data_ptr, tensors))
 
 
-def _table(tensors, with_grads=False):
-    """``(addresses, sizes, addresses of the gradients or None, type code, device index)`` of a list of tensors
-    in one call, or None where they are not all alike (see ``csrc/e2a_torch.cpp``)."""
+def _zeros(typecode, n):
+    return array(typecode, (0,)) * n
+
+
+def _table(tensors):
+    """``(addresses, sizes, type code, device index)`` of a list of tensors in one call, or None where they are
+    not all alike (see ``csrc/e2a_torch.cpp``)."""
     n = len(tensors)
-    at, numel, two = array("Q", (0,)) * n, array("q", (0,)) * n, array("i", (0, 0))
-    grads = array("Q", (0,)) * n if with_grads else None
-    if _lib.load_torch().e2a_tensor_table(tensors, n, _address(at), _address(numel),
-                                            _address(grads) if with_grads else None, _address(two),
-                                            _address(two) + 4):
+    at, numel, two = _zeros("Q", n), _zeros("q", n), _zeros("i", 2)
+    if _lib.load_torch().e2a_tensor_table(tensors, n, _address(at), _address(numel), _address(two), _address(two) + 4):
         return None
-    return at, numel, grads, two[0], two[1]
+    return at, numel, two[0], two[1]
 
 
 def _one_device(tensors, what):
@@ -67,14 +68,14 @@ def _by_type(what, tensors, *others):
 
 
 def _norm(dev, lists):
-    """The norm of ``lists`` = [(type code, addresses, sizes)] of contiguous tensors on the current device."""
+    """The norm of ``lists`` = [(type code, number, addresses, sizes)] of contiguous tensors on the current device."""
     lib, stream = _lib.load(), stream_of(dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    size = sum(lib.e2a_grad_norm_workspace_bytes(len(at)) for _, at, _ in lists)
+    size = sum(lib.e2a_grad_norm_workspace_bytes(n) for _, n, _, _ in lists)
     ws = torch.empty(max(size, 8), dtype=torch.uint8, device=dev)
     base, done, count = ws.data_ptr(), 0, array("q", (0,))
-    for code, at, numel in lists:
-        check(lib.e2a_sum_squares(_address(at), _address(numel), len(at), code, base + 8 * done, size - 8 * done,
+    for code, n, at, numel in lists:
+        check(lib.e2a_sum_squares(_address(at), _address(numel), n, code, base + 8 * done, size - 8 * done,
                                   _address(count), stream), "e2a_sum_squares")
         done += count[0]
     check(lib.e2a_norm_of_squares(base, done, norm.data_ptr(), stream), "e2a_norm_of_squares")
@@ -88,12 +89,12 @@ def grad_norm(tensors):
     tensors = list(tensors)
     found = _table(tensors) if tensors else None
     if found is not None:
-        at, numel, _, code, index = found
-        dev, lists = torch.device("cuda", index), [(code, at, numel)]
+        at, numel, code, index = found
+        dev, lists = torch.device("cuda", index), [(code, len(at), at, numel)]
     else:
         dev = _one_device(tensors, "the tensors") if tensors else torch.device("cuda", torch.cuda.current_device())
         tensors = _contiguous(tensors)
-        lists = [(code, _pointers(ts), array("q", map(torch.Tensor.numel, ts)))
+        lists = [(code, len(ts), _pointers(ts), array("q", map(torch.Tensor.numel, ts)))
                  for code, ts in _by_type("grad_norm", tensors)]
     if dev.index == torch.cuda.current_device():
         return _norm(dev, lists)
@@ -261,7 +262,7 @@ class AdamW(torch.optim.Optimizer):
             if any(w[1].device != dev for w in work):
                 raise ValueError("the parameters to clip together are on more than one device")
             with torch.cuda.device(dev):
-                norm = self.last_grad_norm = _norm(dev, [(w[2], w[4], w[5]) for w in work])
+                norm = self.last_grad_norm = _norm(dev, [(w[2], w[3], w[5], w[6]) for w in work])
         for w in work:
             if w[1].device.index == torch.cuda.current_device():
                 self._launch(*w, norm)
@@ -271,21 +272,33 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _group_work(self, gi, group, keep):
-        """The launches of a group: ``[(group, flat state, type code, addresses of the parameters and of their
-        gradients, sizes, state offsets, slots, parameters)]``; ``keep`` holds what has to live until then."""
+        """The launches of a group: ``[(group, flat state, type code, number of tensors, addresses of the parameters
+        and of their gradients, sizes, state offsets, slots)]``; ``keep`` holds what has to live until then."""
         params = group["params"]
         if not params:
             return []
-        found = _table(params, True)
-        if found is not None:
-            at, numel, grads, code, index = found
+        flat = self._flat.get(gi)
+        if flat is None:
+            if all(p.grad is None for p in params):
+                return []
             flat = self._group_state(gi)
-            if index == flat.device.index and numel == flat.numel:
-                return [(group, flat, code, at, grads, numel, flat.offset, flat.slot, params)]
+        n = len(params)
+        at, grads, numel, offset, slot = (_zeros(t, n) for t in "QQqqi")
+        info = _zeros("i", 3)
+        if n == len(flat.numel) and not _lib.load_torch().e2a_step_table(
+                params, n, _address(flat.numel), _address(flat.offset), _address(at), _address(grads), _address(numel),
+                _address(offset), _address(slot), _address(info), _address(info) + 4, _address(info) + 8):
+            code, index, count = info
+            if count == 0:
+                return []
+            if index != flat.device.index:
+                raise ValueError("the parameters have moved to another device than their state")
+            return [(group, flat, code, count, at, grads, numel, offset, slot)]
+        if n != len(flat.numel):
+            raise ValueError("the group's parameters are not those its state was made for")
         index = [k for k, p in enumerate(params) if p.grad is not None]
         if not index:
             return []
-        flat = self._group_state(gi)
         params = [params[k] for k in index]
         if _one_device(params, "a group's parameters") != flat.device:
             raise ValueError("the parameters have moved to another device than their state")
@@ -295,11 +308,14 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("a parameter has changed its size since its state was made")
         grads = _contiguous([p.grad for p in params])
         keep.append(grads)
-        return [(group, flat, code, _pointers(ps), _pointers(gs), *(
-            array(a.typecode, [a[k] for k in ks]) for a in (flat.numel, flat.offset, flat.slot)), ps)
+        work = [(group, flat, code, len(ps), _pointers(ps), _pointers(gs), *(
+            array(a.typecode, [a[k] for k in ks]) for a in (flat.numel, flat.offset, flat.slot)))
             for code, ps, gs, ks in _by_type("AdamW", params, grads, index)]
+        # the kernels write behind autograd's back: saved tensors and caches keyed on versions have to see it
+        torch.autograd.graph.increment_version(params)
+        return work
 
-    def _launch(self, group, flat, code, at, grads, numel, offset, slot, params, norm):
+    def _launch(self, group, flat, code, count, at, grads, numel, offset, slot, norm):
         lr, lr_at = group["lr"], None
         if isinstance(lr, torch.Tensor) and lr.is_cuda:
             if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != flat.device:
@@ -309,11 +325,9 @@ class AdamW(torch.optim.Optimizer):
         m, v, ms, vs, step = (b[k].data_ptr() if k in b else None for k in (
             "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "step"))
         lib = _lib.load()
-        ws = torch.empty(lib.e2a_adamw_workspace_bytes(len(at)), dtype=torch.uint8, device=flat.device)
+        ws = torch.empty(lib.e2a_adamw_workspace_bytes(count), dtype=torch.uint8, device=flat.device)
         check(lib.e2a_adamw_step(
-            _address(at), _address(grads), _address(numel), _address(offset), _address(slot), len(at), code, flat.bits,
+            _address(at), _address(grads), _address(numel), _address(offset), _address(slot), count, code, flat.bits,
             m, v, ms, vs, flat.elements, step, lr, lr_at, beta1, beta2, group["eps"], group["weight_decay"],
             None if norm is None else norm.data_ptr(), self.max_grad_norm or 0.0, ws.data_ptr(), ws.numel(),
             stream_of(flat.device)), "e2a_adamw_step")
-        # the kernels write behind autograd's back: saved tensors and caches keyed on versions have to see it
-        torch.autograd.graph.increment_version(params)
