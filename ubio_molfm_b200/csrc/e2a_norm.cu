@@ -47,22 +47,7 @@ __device__ __forceinline__ Act activation(float z, bool silu) {
   return {z * s, s * (1.f + z * (1.f - s)), s * (1.f - s) * (2.f + z * (1.f - 2.f * s))};
 }
 
-// The same of two neighbouring values: packed fp32 arithmetic takes one issue slot for both.
-__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float2 f2_mul(float2 a, float2 b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(d)
-      : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
-  return *reinterpret_cast<float2*>(&d);
-}
-__device__ __forceinline__ float2 f2_add(float2 a, float2 b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(d)
-      : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
-  return *reinterpret_cast<float2*>(&d);
-}
+// The same of two neighbouring values in packed fp32 arithmetic.
 __device__ __forceinline__ float2 sigmoid(float2 z) {
   const float2 t = f2_mul(z, f2(-1.44269504f));
   float2 e, s;

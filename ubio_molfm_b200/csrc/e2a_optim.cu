@@ -160,7 +160,13 @@ __device__ __forceinline__ float root_approx(float x) {     // within 2^-23; 0 b
 }
 
 // What all elements of a launch share.
-struct Rates { float b1, a1, b2, a2, eps; };
+struct Rates { float b1, a1, b2, a2, eps, one; };
+
+// a b + c d, each product and the sum rounded on its own.  The sum is a fused product with a 1 that the compiler
+// does not know: it may contract a packed product and sum into one rounding.
+__device__ __forceinline__ float2 sum_of_products(float2 a, float b, float2 c, float d, float one) {
+  return f2_fma(f2_mul(a, f2(b)), f2(one), f2_mul(c, f2(d)));
+}
 
 // One element's moments; every operation rounded on its own (see above).
 __device__ __forceinline__ float next_m(float m, float g, const Rates& r) {
@@ -222,102 +228,145 @@ __device__ __forceinline__ void store8(T* p, int64_t i, int64_t n, bool vec, con
   store4(p, i + 128, n, vec, *reinterpret_cast<const float4*>(v.v + 4));
 }
 
-// Where a warp's block lies and what its tensor shares.
+// Where a thread's values lie: its first element, the tensor's elements, and the bits (element, step) are mixed from.
 struct Where {
-  int64_t i, n;        // the thread's first element, the tensor's elements
-  uint32_t mix;        // i and t's share of the mixed bits
+  int64_t i, n;
+  uint32_t mix;
 };
 
 constexpr uint32_t kMixIndex = 0xDB4F0B91u;
 
-// A thread's share of a block: parameters, codes and shared exponents.
-struct Held {
-  Eight p;
-  uint32_t cm[2], cv[2], em, es;
+// A thread's codes of a block and the block's shared exponents.
+struct Codes {
+  uint32_t m[2], s[2], em, es;
 };
 
-// The step for any values.  By value: the arguments of the rarely made call must not tie the caller's to memory.
-__device__ __noinline__ Held block_exact(const Held h, const Eight g, const Where w, const Globals gl, const Scalars sc,
-                                         const Rates r) {
-  Held o;
+// The new codes for any values, and the new parameters if they are not there yet.  By value, and g read again: the
+// rarely made call must not tie the caller's values to memory or registers.
+template <typename T>
+__device__ __noinline__ Codes block_exact(const Codes h, T* p, const T* g, bool vec, bool with_p, bool clip,
+                                          const Where w, const Globals gl, const Scalars sc, const Rates r) {
   Eight m, s;
+  Eight pv = load8(p, w.i, w.n, vec);
+  const Eight gv = load8(g, w.i, w.n, vec);
   uint32_t top_m = 0, top_s = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float r0 = unpack_s((h.cv[e / 4] >> (8 * (e % 4))) & 255u, scale_of(h.es));
-    m.v[e] = next_m(unpack_m((h.cm[e / 4] >> (8 * (e % 4))) & 255u, scale_of(h.em)), g.v[e], r);
-    s.v[e] = __fsqrt_rn(next_v(__fmul_rn(r0, r0), g.v[e], r));
-    o.p.v[e] = next_p(h.p.v[e], m.v[e], s.v[e], gl, sc, r.eps);
+    const float ge = clip ? __fmul_rn(gv.v[e], gl.coef) : gv.v[e];
+    const float r0 = unpack_s((h.s[e / 4] >> (8 * (e % 4))) & 255u, scale_of(h.es));
+    m.v[e] = next_m(unpack_m((h.m[e / 4] >> (8 * (e % 4))) & 255u, scale_of(h.em)), ge, r);
+    s.v[e] = __fsqrt_rn(next_v(__fmul_rn(r0, r0), ge, r));
+    pv.v[e] = next_p(pv.v[e], m.v[e], s.v[e], gl, sc, r.eps);
     if (w.i + e % 4 + 128 * (e / 4) >= w.n) m.v[e] = s.v[e] = 0.f;     // a block holds no more than its tensor
     top_m = max(top_m, __float_as_uint(m.v[e]) & 0x7FFFFFFFu);
     top_s = max(top_s, __float_as_uint(s.v[e]) & 0x7FFFFFFFu);
   }
+  if (with_p) store8(p, w.i, w.n, vec, pv);
+  Codes o{};
   o.em = shared_exponent(__reduce_max_sync(0xffffffffu, top_m), 3);
   o.es = shared_exponent(__reduce_max_sync(0xffffffffu, top_s), 4);
-  o.cm[0] = o.cm[1] = o.cv[0] = o.cv[1] = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const uint32_t u = mixed(w.mix + (e % 4 + 128 * (e / 4)) * kMixIndex);
-    o.cm[e / 4] |= pack_m(m.v[e], o.em, u >> 12) << (8 * (e % 4));
-    o.cv[e / 4] |= pack_s(s.v[e], o.es, u & 0x7FFFFu) << (8 * (e % 4));
+    o.m[e / 4] |= pack_m(m.v[e], o.em, u >> 12) << (8 * (e % 4));
+    o.s[e / 4] |= pack_s(s.v[e], o.es, u & 0x7FFFFu) << (8 * (e % 4));
   }
   return o;
 }
 
-// The same codes for a whole block of ordinary values in about half the instructions: scales as one product, no
-// clamps, and square roots within 2^-23, whose code is the exact root's unless the rounding offset brings it within
-// a few units of the next one.  False (for all of the warp) where any of this may not hold: block_exact then does
-// it again from h.
-__device__ __forceinline__ bool block_fast(const Held& h, Held& o, const Eight& g, const Where& w, const Globals& gl,
-                                           const Scalars& sc, const Rates& r) {
-  // scales 2^(e + 112) of the old codes, in range for e <= 15; none for a NaN block
-  if (w.i - 4 * (threadIdx.x & 31) + kBlock > w.n || max(h.em, h.es) > 127 + 15) return false;
-  const float fm = __uint_as_float((h.em + 112u) << 23), fs = __uint_as_float((h.es + 112u) << 23);
-  Eight m, s;
-  uint32_t top_m = 0, top_s = 0, alive = 0;
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Byte `k` of a word as its top byte, and four words' top bytes as one word.
+__device__ __forceinline__ uint32_t byte_on_top(uint32_t w, int k) { return __byte_perm(w, 0u, (k << 12) | 0x444u); }
+__device__ __forceinline__ uint32_t top_bytes(const uint32_t* w) {
+  return __byte_perm(__byte_perm(w[0], w[1], 0x0073u), __byte_perm(w[2], w[3], 0x0073u), 0x5410u);
+}
+
+// The step of a whole block of ordinary values, in about half of block_exact's instructions (its time is theirs: 82
+// an element took 408 us on 120M bf16 values, whose bytes take 184): packed fp32 arithmetic, scales as one product,
+// no clamps, and square roots within 2^-23.  A root's code is the exact one's unless the rounding offset brings it
+// within a few units of the next code; where that, or a value's range, is in doubt for any of the warp, `sure` is
+// false and the codes are not to be used.  The parameters are stored either way.
+template <typename T>
+__device__ __forceinline__ Codes block_fast(const Codes& h, T* pt, const T* gt, bool vec, bool clip, const Where& w,
+                                            const Globals& gl, const Scalars& sc, const Rates& r, bool* sure) {
+  // scales 2^(e + 112) of the old codes, in range for e <= 15 (the caller has looked)
+  const float2 fm = f2(__uint_as_float((h.em + 112u) << 23)), fs = f2(__uint_as_float((h.es + 112u) << 23));
+  float2 m[4], s[4];
+  float top_m = 0.f, top_s = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int k = 8 * (e % 4);
-    const uint32_t a = h.cm[e / 4], b = h.cv[e / 4];
-    // magnitude to bits 20..26, sign to bit 31
-    const uint32_t mag = (k <= 20 ? a << (20 - k) : a >> (k - 20)) & 0x07F00000u, sign = (a << (24 - k)) & 0x80000000u;
-    const float m0 = __fmul_rn(__uint_as_float(mag | sign), fm);
-    const float s0 = __fmul_rn(__uint_as_float((k <= 19 ? b << (19 - k) : b >> (k - 19)) & 0x07F80000u), fs);
-    m.v[e] = next_m(m0, g.v[e], r);
-    const float v = next_v(__fmul_rn(s0, s0), g.v[e], r);
-    alive |= (__float_as_uint(v) != 0u ? 1u : 0u) << e;
-    s.v[e] = root_approx(v);
-    o.p.v[e] = next_p(h.p.v[e], m.v[e], s.v[e], gl, sc, r.eps);
-    top_m = max(top_m, __float_as_uint(m.v[e]) & 0x7FFFFFFFu);
-    top_s = max(top_s, __float_as_uint(s.v[e]));
+  for (int half = 0; half < 2; ++half) {
+    float4 p4 = load4(pt, w.i + 128 * half, w.n, vec);
+    const float4 g4 = load4(gt, w.i + 128 * half, w.n, vec);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int e = 2 * half + q;
+      float2 g = q ? make_float2(g4.z, g4.w) : make_float2(g4.x, g4.y);
+      const float2 p = q ? make_float2(p4.z, p4.w) : make_float2(p4.x, p4.y);
+      if (clip) g = f2_mul(g, f2(gl.coef));
+      const uint32_t a0 = byte_on_top(h.m[half], 2 * q), a1 = byte_on_top(h.m[half], 2 * q + 1);
+      const uint32_t b0 = byte_on_top(h.s[half], 2 * q), b1 = byte_on_top(h.s[half], 2 * q + 1);
+      // magnitude to bits 20..26 (19..26), sign to bit 31
+      const float2 m0 = f2_mul(make_float2(__uint_as_float((uint32_t)((int32_t)a0 >> 4) & 0x87F00000u),
+                                           __uint_as_float((uint32_t)((int32_t)a1 >> 4) & 0x87F00000u)), fm);
+      const float2 s0 = f2_mul(make_float2(__uint_as_float(b0 >> 5), __uint_as_float(b1 >> 5)), fs);
+      m[e] = sum_of_products(m0, r.b1, g, r.a1, r.one);
+      const float2 v = sum_of_products(f2_mul(s0, s0), r.b2, f2_mul(g, g), r.a2, r.one);
+      s[e] = make_float2(root_approx(v.x), root_approx(v.y));
+      const float2 d = f2_fma(s[e], f2(sc.root), f2(r.eps));
+      const float2 up = f2_mul(m[e], make_float2(reciprocal(d.x), reciprocal(d.y)));
+      const float2 next = f2_fma(up, f2(-sc.size), f2_mul(p, f2(gl.decay)));
+      if (q) {
+        p4.z = next.x;
+        p4.w = next.y;
+      } else {
+        p4.x = next.x;
+        p4.y = next.y;
+      }
+      top_m = max_or_nan(max_or_nan(top_m, fabsf(m[e].x)), fabsf(m[e].y));
+      top_s = max_or_nan(max_or_nan(top_s, s[e].x), s[e].y);
+    }
+    store4(pt, w.i + 128 * half, w.n, vec, p4);
   }
-  top_m = __reduce_max_sync(0xffffffffu, top_m);
-  top_s = __reduce_max_sync(0xffffffffu, top_s);
-  const uint32_t em = shared_exponent(top_m, 3), es = shared_exponent(top_s, 4);
+  Codes o;
+  const uint32_t bits_s = __reduce_max_sync(0xffffffffu, __float_as_uint(top_s) & 0x7FFFFFFFu);
+  o.em = shared_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m) & 0x7FFFFFFFu), 3);
+  o.es = shared_exponent(bits_s, 4);
   // in range for one product each (NaN and infinities are above), and the exponent not in doubt
-  if (em > 127 + 14 || es > 127 + 14 || es < 127 - 40 || ((top_s + (1u << 19) + 4u) & 0x7FFFFFu) < 8u) return false;
-  const float zm = __uint_as_float((254u - 112u - em) << 23), zs = __uint_as_float((254u - 112u - es) << 23);
-  uint32_t wm[2] = {0, 0}, ws[2] = {0, 0}, doubt = 0;
+  *sure = o.em <= 127 + 14 && o.es <= 127 + 14 && o.es >= 127 - 40 && ((bits_s + (1u << 19) + 4u) & 0x7FFFFFu) >= 8u;
+  if (!*sure) return o;
+  const float zm = __uint_as_float((254u - 112u - o.em) << 23);
+  const float2 zs = f2(__uint_as_float((254u - 112u - o.es) << 23));
+  uint32_t doubt = 8u;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int k = 8 * (e % 4);
-    const uint32_t u = mixed(w.mix + (e % 4 + 128 * (e / 4)) * kMixIndex);
-    const uint32_t bm = __float_as_uint(m.v[e]);
-    const uint32_t tm = __float_as_uint(__fmul_rn(fabsf(m.v[e]), zm)) + (u >> 12);
-    wm[e / 4] |= (tm >> 20) << k | ((bm >> 24) & 128u) << k;
-    const uint32_t ts = __float_as_uint(__fmul_rn(s.v[e], zs)) + (u & 0x7FFFFu);
-    doubt |= ((ts + 4u) & 0x7FFFFu) < 8u ? 1u : 0u;
-    ws[e / 4] |= max(ts >> 19, (alive >> e) & 1u) << k;
-  }
-  if (__any_sync(0xffffffffu, doubt)) return false;
+  for (int half = 0; half < 2; ++half) {
+    uint32_t cm[4], cs[4];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    o.cm[k] = wm[k];
-    o.cv[k] = ws[k];
+    for (int q = 0; q < 2; ++q) {
+      const float2 mv = m[2 * half + q], sv = s[2 * half + q], z = f2_mul(sv, zs);
+      const float me[2] = {mv.x, mv.y}, se[2] = {sv.x, sv.y}, ze[2] = {z.x, z.y};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t u = mixed(w.mix + (2 * q + k + 128 * half) * kMixIndex);
+        const uint32_t tm = __float_as_uint(__fmul_rn(fabsf(me[k]), zm)) + (u >> 12);
+        cm[2 * q + k] = (tm << 4) | (__float_as_uint(me[k]) & 0x80000000u);
+        // over zero at least the smallest code (a root of a subnormal, 0 here, counts as zero); 4 more than the
+        // sum, so that what is in doubt lies in 0..7 of the dropped bits
+        const float least = fminf(se[k], __uint_as_float(1u << 19));
+        const uint32_t ts = __float_as_uint(fmaxf(ze[k], least)) + (u & 0x7FFFFu) + 4u;
+        doubt = min(doubt, ts & 0x7FFFFu);
+        cs[2 * q + k] = ts << 5;
+      }
+    }
+    o.m[half] = top_bytes(cm);
+    o.s[half] = top_bytes(cs);
   }
-  o.em = em;
-  o.es = es;
-  return true;
+  *sure = !__any_sync(0xffffffffu, doubt < 8u);
+  return o;
 }
 
 // A CTA walks a contiguous range of units; a warp owns one block of 256 of each, lane l the values 4 l and
@@ -339,9 +388,10 @@ k_adamw(const __grid_constant__ Table tab, int32_t n_units, int32_t per_cta, voi
     const int64_t i = i0 + 4 * lane, at = tab.offset[j] + i;
     const Scalars s = scal[j];
     T* pt = reinterpret_cast<T*>(tab.p[j]);
+    const T* gt = reinterpret_cast<const T*>(tab.g[j]);
     const bool vec = ((tab.p[j] | tab.g[j]) & (4 * sizeof(T) - 1)) == 0;
-    Eight p = load8(pt, i, n, vec), g = load8(reinterpret_cast<const T*>(tab.g[j]), i, n, vec);
     if (BITS == 32) {
+      Eight p = load8(pt, i, n, vec), g = load8(gt, i, n, vec);
       float* mt = (float*)exp_avg + at;
       float* vt = (float*)exp_avg_sq + at;
       Eight m, v;
@@ -366,19 +416,18 @@ k_adamw(const __grid_constant__ Table tab, int32_t n_units, int32_t per_cta, voi
     } else {
       uint32_t* mt = reinterpret_cast<uint32_t*>((uint8_t*)exp_avg + at);
       uint32_t* vt = reinterpret_cast<uint32_t*>((uint8_t*)exp_avg_sq + at);
-      const Held h{p, {mt[0], mt[32]}, {vt[0], vt[32]}, scale_m[at / kBlock], scale_v[at / kBlock]};
-      Held o;
-      if (clip) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) g.v[e] = __fmul_rn(g.v[e], gl.coef);
-      }
+      const Codes h{{mt[0], mt[32]}, {vt[0], vt[32]}, scale_m[at / kBlock], scale_v[at / kBlock]};
       const Where w{i, n, (uint32_t)i * kMixIndex + (uint32_t)s.t * 0xBBE05633u};
-      if (!block_fast(h, o, g, w, gl, s, r)) o = block_exact(h, g, w, gl, s, r);
-      store8(pt, i, n, vec, o.p);
-      mt[0] = o.cm[0];
-      mt[32] = o.cm[1];
-      vt[0] = o.cv[0];
-      vt[32] = o.cv[1];
+      // whole blocks of moments below 2^16; a block of NaN has exponent 255
+      const bool ordinary = i0 + kBlock <= n && max(h.em, h.es) <= 127 + 15;
+      bool sure = false;
+      Codes o;
+      if (ordinary) o = block_fast(h, pt, gt, vec, clip, w, gl, s, r, &sure);
+      if (!sure) o = block_exact(h, pt, gt, vec, !ordinary, clip, w, gl, s, r);
+      mt[0] = o.m[0];
+      mt[32] = o.m[1];
+      vt[0] = o.s[0];
+      vt[32] = o.s[1];
       if (lane == 0) {
         scale_m[at / kBlock] = (uint8_t)o.em;
         scale_v[at / kBlock] = (uint8_t)o.es;
@@ -639,7 +688,7 @@ int e2a_adamw_step(const uint64_t* params, const uint64_t* grads, const int64_t*
   Scalars* scal = (Scalars*)(glob + 1);
   cudaStream_t st = (cudaStream_t)stream;
   const Hyper h{lr, std::log2(beta1), std::log2(beta2), weight_decay, lr_device, grad_norm, (float)max_norm};
-  const Rates r{(float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps};
+  const Rates r{(float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps, 1.f};
   for (int64_t j = 0; j < n_tensors;) {
     static thread_local Table t;
     static thread_local Slots slot;
