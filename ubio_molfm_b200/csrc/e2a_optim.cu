@@ -34,7 +34,9 @@ constexpr int kThreads = 256;
 constexpr int kUnit = 8 * kBlock;    // elements that a CTA takes at a time: one block a warp
 constexpr int kTensors = 512;        // tensors in one launch's table (18.4 KB of kernel parameters)
 constexpr int kNormCtas = 1184;      // partial sums of squares of one launch (8 per SM)
-constexpr int kStepCtas = 148 * 16;  // CTAs of one step: contiguous ranges, a few waves so that they even out
+// CTAs of one step, each a contiguous range: a few waves so that they even out; with 8 bits one wave, whose start
+// (its tensor, its scalars) then counts once (24.5M fp32 parameters: 16 a SM 126 us, 4 a SM 94 us)
+constexpr int kStepCtas32 = 148 * 16, kStepCtas8 = 148 * 4;
 
 struct Table {
   uint64_t p[kTensors];
@@ -702,7 +704,7 @@ int e2a_adamw_step(const uint64_t* params, const uint64_t* grads, const int64_t*
     rc = by_type(dtype, [&](auto* x) -> int {
       using T = std::remove_pointer_t<decltype(x)>;
       auto* kernel = state_bits == 32 ? k_adamw<T, 32> : k_adamw<T, 8>;
-      const int32_t per = (units + kStepCtas - 1) / kStepCtas, ctas = (units + per - 1) / per;
+      const int32_t most = state_bits == 32 ? kStepCtas32 : kStepCtas8, per = (units + most - 1) / most, ctas = (units + per - 1) / per;
       kernel<<<ctas, kThreads, 0, st>>>(t, units, per, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale,
                                         scal + from, glob, r, grad_norm != nullptr);
       E2A_CHECK_LAUNCH();
