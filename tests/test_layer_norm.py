@@ -333,6 +333,9 @@ def test_constant_rows_and_no_rows():
     w, b = torch.full((32,), 2.0, device=DEV), torch.full((32,), 0.5, device=DEV)
     y = layer_norm(torch.full((3, 32), 7.0, device=DEV), w, b, EPS)
     assert bool((y == 0.5).all())             # variance 0: xh is 0 exactly
+    for width in (3, 12, 100, 1000, 5000):    # 7 k is exact, and so is the mean
+        y = layer_norm(torch.full((2, width), 7.0, device=DEV), bias=torch.full((width,), 0.5, device=DEV))
+        assert bool((y == 0.5).all()), width
     x = torch.zeros(0, 32, device=DEV, requires_grad=True)
     w.requires_grad_(True)
     y = layer_norm(x, w, b, EPS)

@@ -554,6 +554,66 @@ def test_other_stream_and_other_layouts():
         AdamW([w]).step()
 
 
+@pytest.mark.gpu
+def test_learning_rates_as_tensors_and_schedules():
+    from ubio_molfm_b200.optim import AdamW
+
+    a, b, c = (_params([500], torch.float32, 13) for _ in range(3))
+    oa, ob = AdamW(a, lr=2e-3), AdamW(b, lr=torch.tensor(2e-3))
+    oc = AdamW(c, lr=4e-3)
+    torch.optim.lr_scheduler.LambdaLR(oc, lambda epoch: 0.5)          # takes the optimiser, sets lr to 2e-3
+    for o in (oa, ob, oc):
+        o.step()
+    assert torch.equal(a[0], c[0])
+    # 2e-3 as a float32 tensor is off by at most 2^-24 of itself, and so is the update of at most 2e-3
+    assert float((a[0] - b[0]).detach().abs().max()) <= 2e-3 * 2 * U + 2 * U * float(a[0].detach().abs().max())
+    d = _params([8], torch.float32, 1)
+    with pytest.raises(ValueError, match="lr"):
+        AdamW(d, lr=torch.tensor(1e-3, dtype=torch.float64, device=DEV)).step()
+
+
+@pytest.mark.gpu
+def test_sparse_gradients_are_refused():
+    from ubio_molfm_b200.optim import AdamW, grad_norm
+
+    e = torch.nn.Embedding(10, 4, sparse=True).to(DEV)
+    e(torch.tensor([1, 2], device=DEV)).sum().backward()
+    with pytest.raises(TypeError):
+        AdamW(e.parameters()).step()
+    with pytest.raises(TypeError):
+        grad_norm([e.weight.grad])
+
+
+@pytest.mark.gpu
+def test_more_than_2_to_the_32_elements():
+    """Elements 2^32 apart have the same mixed bits: with the same values in every block of 256, the block that
+    starts there becomes what the first one becomes."""
+    from ubio_molfm_b200.optim import AdamW, grad_norm
+
+    n, tail = (1 << 32) + 256 * 3 + 100, 256
+    block = torch.randn(256, device=DEV).bfloat16()
+    p = torch.nn.Parameter(torch.empty(n, dtype=torch.bfloat16, device=DEV))
+    whole = n // 256 * 256
+    with torch.no_grad():
+        p[:whole].view(-1, 256).copy_(block)
+        p[whole:] = block[:n - whole]
+    p.grad = p.detach().clone()
+    want = math.sqrt(float(block.double().square().sum()) * (n // 256) + float(block[:n - whole].double().square().sum()))
+    assert abs(float(grad_norm([p.grad])) - want) <= (U + 1e-9) * want
+    opt = AdamW([p], lr=1e-2, state_bits=8)
+    for _ in range(2):
+        opt.step()
+    st = opt.flat_state()
+    at = 1 << 32
+    assert torch.equal(p[at:at + tail], p[:tail]) and not torch.equal(p[:tail].detach(), block)
+    for k in ("exp_avg", "exp_avg_sq"):
+        assert torch.equal(st[k][at:at + tail], st[k][:tail])
+        assert not bool(st[k][n:].any())
+    # the last block, cut short: its moments have the first one's values or, where its largest value is smaller,
+    # a smaller scale; its parameters do not depend on that after one step more than the moments' own rounding
+    assert bool(torch.isfinite(p[-100:]).all()) and not torch.equal(p[-100:].detach(), block[:100])
+
+
 # ------------------------------------------------------------------------------------------------
 # the norm
 # ------------------------------------------------------------------------------------------------

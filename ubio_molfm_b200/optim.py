@@ -321,6 +321,8 @@ class AdamW(torch.optim.Optimizer):
             if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != flat.device:
                 raise ValueError("a tensor lr must be one float32 value on the parameters' device")
             lr, lr_at = 0.0, lr.data_ptr()
+        else:
+            lr = float(lr)
         (beta1, beta2), b = group["betas"], flat.buffers
         m, v, ms, vs, step = (b[k].data_ptr() if k in b else None for k in (
             "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "step"))
