@@ -162,7 +162,12 @@ __device__ __forceinline__ float root_approx(float x) {     // within 2^-23; 0 b
 }
 
 // What all elements of a launch share.
-struct Rates { float b1, a1, b2, a2, eps, one; };
+struct Rates {
+  float b1, a1, b2, a2, eps, one;
+  // powers of two that the compiler does not know: shifts by them are products, on the multiplying pipe, where the
+  // integer pipe is the one that is full
+  uint32_t two[6], x1, x16, x32;
+};
 
 // a b + c d, each product and the sum rounded on its own.  The sum is a fused product with a 1 that the compiler
 // does not know: it may contract a packed product and sum into one rounding.
@@ -276,14 +281,13 @@ __device__ __noinline__ Codes block_exact(const Codes h, T* p, const T* g, bool 
   return o;
 }
 
-__device__ __forceinline__ float max_or_nan(float a, float b) {
+__device__ __forceinline__ float max_or_nan(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
-// Byte `k` of a word as its top byte, and four words' top bytes as one word.
-__device__ __forceinline__ uint32_t byte_on_top(uint32_t w, int k) { return __byte_perm(w, 0u, (k << 12) | 0x444u); }
+// Four words' top bytes as one word.
 __device__ __forceinline__ uint32_t top_bytes(const uint32_t* w) {
   return __byte_perm(__byte_perm(w[0], w[1], 0x0073u), __byte_perm(w[2], w[3], 0x0073u), 0x5410u);
 }
@@ -310,12 +314,14 @@ __device__ __forceinline__ Codes block_fast(const Codes& h, T* pt, const T* gt, 
       float2 g = q ? make_float2(g4.z, g4.w) : make_float2(g4.x, g4.y);
       const float2 p = q ? make_float2(p4.z, p4.w) : make_float2(p4.x, p4.y);
       if (clip) g = f2_mul(g, f2(gl.coef));
-      const uint32_t a0 = byte_on_top(h.m[half], 2 * q), a1 = byte_on_top(h.m[half], 2 * q + 1);
-      const uint32_t b0 = byte_on_top(h.s[half], 2 * q), b1 = byte_on_top(h.s[half], 2 * q + 1);
-      // magnitude to bits 20..26 (19..26), sign to bit 31
+      // bytes 2 q and 2 q + 1 of the codes: to the top, from there the magnitude to bits 20..26 with the sign staying
+      // in 31; the second moment's to bits 19..26 (its last byte is the one that moves down)
+      const uint32_t a0 = h.m[half] * r.two[q ? 2 : 0], a1 = q ? h.m[half] : h.m[half] * r.two[1];
+      const uint32_t b0 = h.s[half] * r.two[q ? 5 : 3] & 0x07F80000u;
+      const uint32_t b1 = q ? h.s[half] >> 5 & 0x07F80000u : h.s[half] * r.two[4] & 0x07F80000u;
       const float2 m0 = f2_mul(make_float2(__uint_as_float((uint32_t)((int32_t)a0 >> 4) & 0x87F00000u),
                                            __uint_as_float((uint32_t)((int32_t)a1 >> 4) & 0x87F00000u)), fm);
-      const float2 s0 = f2_mul(make_float2(__uint_as_float(b0 >> 5), __uint_as_float(b1 >> 5)), fs);
+      const float2 s0 = f2_mul(make_float2(__uint_as_float(b0), __uint_as_float(b1)), fs);
       m[e] = sum_of_products(m0, r.b1, g, r.a1, r.one);
       const float2 v = sum_of_products(f2_mul(s0, s0), r.b2, f2_mul(g, g), r.a2, r.one);
       s[e] = make_float2(root_approx(v.x), root_approx(v.y));
@@ -329,8 +335,8 @@ __device__ __forceinline__ Codes block_fast(const Codes& h, T* pt, const T* gt, 
         p4.x = next.x;
         p4.y = next.y;
       }
-      top_m = max_or_nan(max_or_nan(top_m, fabsf(m[e].x)), fabsf(m[e].y));
-      top_s = max_or_nan(max_or_nan(top_s, s[e].x), s[e].y);
+      top_m = max_or_nan(top_m, fabsf(m[e].x), fabsf(m[e].y));
+      top_s = max_or_nan(top_s, s[e].x, s[e].y);
     }
     store4(pt, w.i + 128 * half, w.n, vec, p4);
   }
@@ -353,15 +359,15 @@ __device__ __forceinline__ Codes block_fast(const Codes& h, T* pt, const T* gt, 
       const float me[2] = {mv.x, mv.y}, se[2] = {sv.x, sv.y}, ze[2] = {z.x, z.y};
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const uint32_t u = mixed(w.mix + (2 * q + k + 128 * half) * kMixIndex);
+        const uint32_t u = mixed(w.mix * r.x1 + (2 * q + k + 128 * half) * kMixIndex);
         const uint32_t tm = __float_as_uint(__fmul_rn(fabsf(me[k]), zm)) + (u >> 12);
-        cm[2 * q + k] = (tm << 4) | (__float_as_uint(me[k]) & 0x80000000u);
+        cm[2 * q + k] = (tm * r.x16) | (__float_as_uint(me[k]) & 0x80000000u);
         // over zero at least the smallest code (a root of a subnormal, 0 here, counts as zero); 4 more than the
         // sum, so that what is in doubt lies in 0..7 of the dropped bits
         const float least = fminf(se[k], __uint_as_float(1u << 19));
         const uint32_t ts = __float_as_uint(fmaxf(ze[k], least)) + (u & 0x7FFFFu) + 4u;
         doubt = min(doubt, ts & 0x7FFFFu);
-        cs[2 * q + k] = ts << 5;
+        cs[2 * q + k] = ts * r.x32;
       }
     }
     o.m[half] = top_bytes(cm);
@@ -369,6 +375,18 @@ __device__ __forceinline__ Codes block_fast(const Codes& h, T* pt, const T* gt, 
   }
   *sure = !__any_sync(0xffffffffu, doubt < 8u);
   return o;
+}
+
+// Asks for a later block's lines, a lane each: parameters, gradients and codes.
+template <typename T>
+__device__ __forceinline__ void prefetch_block(const T* p, const T* g, const uint8_t* m, const uint8_t* s) {
+  constexpr int LINES = kBlock * (int)sizeof(T) / 128;
+  const int lane = threadIdx.x & 31;
+  const char* at = lane < LINES ? (const char*)p + lane * 128
+                   : lane < 2 * LINES ? (const char*)g + (lane - LINES) * 128
+                   : lane < 2 * LINES + 2 ? (const char*)m + (lane - 2 * LINES) * 128
+                                          : (const char*)s + (lane - 2 * LINES - 2) * 128;
+  if (lane < 2 * LINES + 4) asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
 }
 
 // A CTA walks a contiguous range of units; a warp owns one block of 256 of each, lane l the values 4 l and
@@ -419,6 +437,9 @@ k_adamw(const __grid_constant__ Table tab, int32_t n_units, int32_t per_cta, voi
       uint32_t* mt = reinterpret_cast<uint32_t*>((uint8_t*)exp_avg + at);
       uint32_t* vt = reinterpret_cast<uint32_t*>((uint8_t*)exp_avg_sq + at);
       const Codes h{{mt[0], mt[32]}, {vt[0], vt[32]}, scale_m[at / kBlock], scale_v[at / kBlock]};
+      if (i0 + kUnit + kBlock <= n)      // the warp's next block
+        prefetch_block(pt + i0 + kUnit, gt + i0 + kUnit, (const uint8_t*)exp_avg + (at - 4 * lane) + kUnit,
+                       (const uint8_t*)exp_avg_sq + (at - 4 * lane) + kUnit);
       const Where w{i, n, (uint32_t)i * kMixIndex + (uint32_t)s.t * 0xBBE05633u};
       // whole blocks of moments below 2^16; a block of NaN has exponent 255
       const bool ordinary = i0 + kBlock <= n && max(h.em, h.es) <= 127 + 15;
@@ -690,7 +711,8 @@ int e2a_adamw_step(const uint64_t* params, const uint64_t* grads, const int64_t*
   Scalars* scal = (Scalars*)(glob + 1);
   cudaStream_t st = (cudaStream_t)stream;
   const Hyper h{lr, std::log2(beta1), std::log2(beta2), weight_decay, lr_device, grad_norm, (float)max_norm};
-  const Rates r{(float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps, 1.f};
+  const Rates r{(float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps, 1.f,
+                {1u << 24, 1u << 16, 1u << 8, 1u << 19, 1u << 11, 1u << 3}, 1u, 16u, 32u};
   for (int64_t j = 0; j < n_tensors;) {
     static thread_local Table t;
     static thread_local Slots slot;
