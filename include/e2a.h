@@ -17,6 +17,7 @@
  *   e2a_alpha_sum_*      sparse_alpha_sum_edge_index_triton      e2f/triton_dr/sparse_alpha_sum_edge_index_autograd.py:207-213
  *   e2a_v_agg_*          sparse_v_agg_edge_index_triton_cblocked e2f/triton_dr/sparse_v_agg_edge_index_cblocked_bench.py:428-449
  *   e2a_edge_outer_*     edge_degree_outer_triton                e2f/triton_dr/edge_degree_outer_autograd.py:348-375
+ *   e2a_layer_norm_*     nn.LayerNorm + nn.SiLU in training      e2f/module_utils.py:2151-2178, 2240-2274
  *   e2a_attn_fwd         E2AttentionArbOrder_sparse.forward, QK logits -> segmented softmax ->
  *                        alpha/r -> value aggregation            e2f/e2former.py:311-364, 393-422;
  *                                                                e2f/wigner6j/so2_tensor_product.py:370-377
@@ -409,7 +410,8 @@ int e2a_layer_norm_bwd2(const void* x, int64_t ldx, const void* dy, int64_t lddy
 /* state_bits 8: one byte an element and, per 256 of them, one scale byte: x = y 2^(scale - 127) with   */
 /* y a small float, m: sign, 4 exponent, 3 fraction bits; sqrt(v): 4 exponent, 4 fraction bits; exponent */
 /* 15 stands for [1, 2), 0 for the subnormals; scale 255 for a block of NaN.  e2a_moments_unpack gives   */
-/* m and v of n elements (whole blocks) as fp32.  Tensors that overlap a parameter are refused (E2A_ERR_ARG).          */
+/* m and v of n elements (whole blocks) as fp32.  Parameters that share memory with another parameter or  */
+/* a gradient are refused (E2A_ERR_ARG).                                                              */
 /* ------------------------------------------------------------------------------------------ */
 size_t e2a_grad_norm_workspace_bytes(int64_t n_tensors);
 int e2a_sum_squares(const uint64_t* tensors, const int64_t* numel, int64_t n_tensors, int dtype, void* workspace,

@@ -17,6 +17,10 @@
 // (an additive sequence in place of mixed bits locks to the value that it rounds: an average that grows by 1e-3
 // a step fell 6% behind in 2,000 steps).  sqrt(v) > 0 is never rounded to 0 (the update would divide by eps).
 // The moments' operations are single rounded fp32 ones in a fixed order, so the codes are reproducible bit for bit.
+//
+// With 32-bit moments it is bound by memory: 24.5M fp32 parameters in 240 tensors (28 bytes each) take 99 us, 6.9 TB/s.
+// With 8-bit ones (16 bytes) 84 us where the bytes take 60; 120M bf16 parameters (10 bytes) 345 us where they take 184:
+// 62 instructions an element keep the integer pipe two thirds busy.  The clipping norm of the 24.5M takes 21 to 27 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -162,12 +166,7 @@ __device__ __forceinline__ float root_approx(float x) {     // within 2^-23; 0 b
 }
 
 // What all elements of a launch share.
-struct Rates {
-  float b1, a1, b2, a2, eps, one;
-  // powers of two that the compiler does not know: shifts by them are products, on the multiplying pipe, where the
-  // integer pipe is the one that is full
-  uint32_t two[6], x1, x16, x32;
-};
+struct Rates { float b1, a1, b2, a2, eps, one; };
 
 // a b + c d, each product and the sum rounded on its own.  The sum is a fused product with a 1 that the compiler
 // does not know: it may contract a packed product and sum into one rounding.
@@ -287,13 +286,14 @@ __device__ __forceinline__ float max_or_nan(float a, float b, float c) {
   return r;
 }
 
-// Four words' top bytes as one word.
+// Byte `k` of a word as its top byte, and four words' top bytes as one word.
+__device__ __forceinline__ uint32_t byte_on_top(uint32_t w, int k) { return __byte_perm(w, 0u, (k << 12) | 0x444u); }
 __device__ __forceinline__ uint32_t top_bytes(const uint32_t* w) {
   return __byte_perm(__byte_perm(w[0], w[1], 0x0073u), __byte_perm(w[2], w[3], 0x0073u), 0x5410u);
 }
 
 // The step of a whole block of ordinary values, in about half of block_exact's instructions (its time is theirs: 82
-// an element took 408 us on 120M bf16 values, whose bytes take 184): packed fp32 arithmetic, scales as one product,
+// an element took 408 us on 120M bf16 values, 62 take 345): packed fp32 arithmetic, scales as one product,
 // no clamps, and square roots within 2^-23.  A root's code is the exact one's unless the rounding offset brings it
 // within a few units of the next code; where that, or a value's range, is in doubt for any of the warp, `sure` is
 // false and the codes are not to be used.  The parameters are stored either way.
@@ -314,11 +314,9 @@ __device__ __forceinline__ Codes block_fast(const Codes& h, T* pt, const T* gt, 
       float2 g = q ? make_float2(g4.z, g4.w) : make_float2(g4.x, g4.y);
       const float2 p = q ? make_float2(p4.z, p4.w) : make_float2(p4.x, p4.y);
       if (clip) g = f2_mul(g, f2(gl.coef));
-      // bytes 2 q and 2 q + 1 of the codes: to the top, from there the magnitude to bits 20..26 with the sign staying
-      // in 31; the second moment's to bits 19..26 (its last byte is the one that moves down)
-      const uint32_t a0 = h.m[half] * r.two[q ? 2 : 0], a1 = q ? h.m[half] : h.m[half] * r.two[1];
-      const uint32_t b0 = h.s[half] * r.two[q ? 5 : 3] & 0x07F80000u;
-      const uint32_t b1 = q ? h.s[half] >> 5 & 0x07F80000u : h.s[half] * r.two[4] & 0x07F80000u;
+      const uint32_t a0 = byte_on_top(h.m[half], 2 * q), a1 = byte_on_top(h.m[half], 2 * q + 1);
+      const uint32_t b0 = byte_on_top(h.s[half], 2 * q) >> 5, b1 = byte_on_top(h.s[half], 2 * q + 1) >> 5;
+      // magnitude to bits 20..26 (19..26), sign to bit 31
       const float2 m0 = f2_mul(make_float2(__uint_as_float((uint32_t)((int32_t)a0 >> 4) & 0x87F00000u),
                                            __uint_as_float((uint32_t)((int32_t)a1 >> 4) & 0x87F00000u)), fm);
       const float2 s0 = f2_mul(make_float2(__uint_as_float(b0), __uint_as_float(b1)), fs);
@@ -359,15 +357,15 @@ __device__ __forceinline__ Codes block_fast(const Codes& h, T* pt, const T* gt, 
       const float me[2] = {mv.x, mv.y}, se[2] = {sv.x, sv.y}, ze[2] = {z.x, z.y};
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const uint32_t u = mixed(w.mix * r.x1 + (2 * q + k + 128 * half) * kMixIndex);
+        const uint32_t u = mixed(w.mix + (2 * q + k + 128 * half) * kMixIndex);
         const uint32_t tm = __float_as_uint(__fmul_rn(fabsf(me[k]), zm)) + (u >> 12);
-        cm[2 * q + k] = (tm * r.x16) | (__float_as_uint(me[k]) & 0x80000000u);
+        cm[2 * q + k] = (tm << 4) | (__float_as_uint(me[k]) & 0x80000000u);
         // over zero at least the smallest code (a root of a subnormal, 0 here, counts as zero); 4 more than the
         // sum, so that what is in doubt lies in 0..7 of the dropped bits
         const float least = fminf(se[k], __uint_as_float(1u << 19));
         const uint32_t ts = __float_as_uint(fmaxf(ze[k], least)) + (u & 0x7FFFFu) + 4u;
         doubt = min(doubt, ts & 0x7FFFFu);
-        cs[2 * q + k] = ts * r.x32;
+        cs[2 * q + k] = ts << 5;
       }
     }
     o.m[half] = top_bytes(cm);
@@ -711,8 +709,7 @@ int e2a_adamw_step(const uint64_t* params, const uint64_t* grads, const int64_t*
   Scalars* scal = (Scalars*)(glob + 1);
   cudaStream_t st = (cudaStream_t)stream;
   const Hyper h{lr, std::log2(beta1), std::log2(beta2), weight_decay, lr_device, grad_norm, (float)max_norm};
-  const Rates r{(float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps, 1.f,
-                {1u << 24, 1u << 16, 1u << 8, 1u << 19, 1u << 11, 1u << 3}, 1u, 16u, 32u};
+  const Rates r{(float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps, 1.f};
   for (int64_t j = 0; j < n_tensors;) {
     static thread_local Table t;
     static thread_local Slots slot;
