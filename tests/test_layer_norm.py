@@ -169,7 +169,10 @@ def test_c_abi_refuses_bad_arguments():
     lib = _lib.load()
     d = ctypes.c_void_p(4096)
     fwd, bwd, bwd2 = lib.e2a_layer_norm_fwd, lib.e2a_layer_norm_bwd, lib.e2a_layer_norm_bwd2
-    ok = lambda rows=4, W=8, ldx=8, dtype=0, act=0, x=d: fwd(x, ldx, dtype, None, None, rows, W, EPS, act, d, d, d, None)  # noqa: E731
+
+    def ok(rows=4, W=8, ldx=8, dtype=0, act=0, x=d):
+        return fwd(x, ldx, dtype, None, None, rows, W, EPS, act, d, d, d, None)
+
     assert ok(rows=0) == 0
     assert ok(rows=-1) == 1 and ok(W=0) == 1 and ok(ldx=-1) == 1 and ok(act=2) == 1 and ok(x=None) == 1
     assert ok(dtype=3) == 1 and ok(dtype=3, rows=0) == 1
@@ -292,6 +295,22 @@ def test_affine_forms(affine):
     (dx,) = torch.autograd.grad(y, xi, gi, create_graph=True)
     for n, t in zip(["g"] + names, torch.autograd.grad(dx, [gi] + leaves, u)):
         _close(t, ref["g" + n], major["g" + n], "g" + n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [96, 77, 9001])
+def test_column_gradients_alone(width):
+    """An input without gradient (the first layer's): only dw and db are formed, and they are the same."""
+    from ubio_molfm_b200.norm import layer_norm
+
+    x, w, b, g, u, p, q = _inputs(70, width, torch.float32)
+    want = _run(x, w, b, True, g)
+    wi, bi = w.clone().requires_grad_(True), b.clone().requires_grad_(True)
+    layer_norm(x, wi, bi, EPS, "silu").backward(g)
+    assert torch.equal(wi.grad, want["dw"]) and torch.equal(bi.grad, want["db"])
+    (db,) = torch.autograd.grad(layer_norm(x, None, bi, EPS), bi, g)
+    ref, major = reference(x, torch.ones_like(w), b, False, g), _majorants(x, torch.ones_like(w), b, g)
+    _close(db, ref["db"], major["db"], "db")
 
 
 @pytest.mark.gpu

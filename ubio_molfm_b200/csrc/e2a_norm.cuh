@@ -141,9 +141,6 @@ __global__ void k_ln_bwd(const T* __restrict__ x, int64_t ldx, const T* __restri
   }
 }
 
-// The row means the second order needs: {<u>, <u xh>, <h>, <h xh>, <h u>} and, from them, t.
-struct RowMeans { float u, c, h1, h2, ht; };
-
 template <typename T>
 __global__ void k_ln_bwd2(const T* __restrict__ x, int64_t ldx, const T* __restrict__ g, int64_t ldg,
                           const T* __restrict__ u, int64_t ldu, Norm n, const float* __restrict__ mean_in,
@@ -257,7 +254,9 @@ __global__ void k_ln_cols_sum(const double* __restrict__ part, int64_t chunks, i
 template <typename T, int VEC> struct Pack;
 template <> struct Pack<float, 4> {
   using Raw = float4;
-  static __device__ __forceinline__ void widen(const Raw& t, float* v) { v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w; }
+  static __device__ __forceinline__ void widen(const Raw& t, float* v) {
+    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+  }
   static __device__ __forceinline__ Raw narrow(const float* v) { return make_float4(v[0], v[1], v[2], v[3]); }
 };
 template <typename T, typename T2> struct Pack16 {
@@ -843,8 +842,8 @@ bool bad_shape(int64_t rows, int64_t W, int64_t ld) { return rows < 0 || W <= 0 
 bool bad_mode(int dtype, int act) { return dtype < 0 || dtype > 2 || (act != 0 && act != 1); }
 
 size_t part_bytes(int64_t rows, int64_t W) {
-  return e2a_align_up(W <= kMaxTeamWidth ? (size_t)most_parts(rows, W) * 2 * W * 4 : (size_t)chunk_count(rows) * 2 * W * 8,
-                      256);
+  return e2a_align_up(W <= kMaxTeamWidth ? (size_t)most_parts(rows, W) * 2 * W * 4
+                                         : (size_t)chunk_count(rows) * 2 * W * 8, 256);
 }
 
 template <typename F>

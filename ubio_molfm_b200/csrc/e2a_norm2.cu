@@ -4,7 +4,8 @@
 extern "C" {
 
 size_t e2a_layer_norm_bwd2_workspace_bytes(int64_t rows, int64_t W) {
-  return rows <= 0 || W <= 0 ? 0 : part_bytes(rows, W) + 2 * e2a_align_up((size_t)rows * sizeof(float), 256);
+  if (rows <= 0 || W <= 0) return 0;
+  return part_bytes(rows, W) + (W <= kMaxTeamWidth ? 0 : 2 * e2a_align_up((size_t)rows * sizeof(float), 256));
 }
 
 int e2a_layer_norm_bwd2(const void* x, int64_t ldx, const void* dy, int64_t lddy, const void* u, int64_t ldu, int dtype,
@@ -17,9 +18,10 @@ int e2a_layer_norm_bwd2(const void* x, int64_t ldx, const void* dy, int64_t lddy
   if (!x || !dy || !u || !mean || !rstd || !d_dy || !dx) return E2A_ERR_ARG;
   E2aArena ar{(char*)workspace, workspace_bytes, 0};
   double* part = (double*)ar.take(part_bytes(rows, W));
-  float* row_u = (float*)ar.take(rows * sizeof(float));
-  float* row_c = (float*)ar.take(rows * sizeof(float));
-  if (!part || !row_u || !row_c) return E2A_ERR_WORKSPACE;
+  const bool loops = W > kMaxTeamWidth;      // <u> and c of every row, for the column sums' own pass
+  float* row_u = loops ? (float*)ar.take(rows * sizeof(float)) : nullptr;
+  float* row_c = loops ? (float*)ar.take(rows * sizeof(float)) : nullptr;
+  if (!part || (loops && (!row_u || !row_c))) return E2A_ERR_WORKSPACE;
   const Norm n{gamma, beta, p, q, W, act == 1};
   return by_type(dtype, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;

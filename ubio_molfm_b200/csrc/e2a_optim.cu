@@ -723,7 +723,8 @@ int e2a_adamw_step(const uint64_t* params, const uint64_t* grads, const int64_t*
     rc = by_type(dtype, [&](auto* x) -> int {
       using T = std::remove_pointer_t<decltype(x)>;
       auto* kernel = state_bits == 32 ? k_adamw<T, 32> : k_adamw<T, 8>;
-      const int32_t most = state_bits == 32 ? kStepCtas32 : kStepCtas8, per = (units + most - 1) / most, ctas = (units + per - 1) / per;
+      const int32_t most = state_bits == 32 ? kStepCtas32 : kStepCtas8;
+      const int32_t per = (units + most - 1) / most, ctas = (units + per - 1) / per;
       kernel<<<ctas, kThreads, 0, st>>>(t, units, per, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale,
                                         scal + from, glob, r, grad_norm != nullptr);
       E2A_CHECK_LAUNCH();

@@ -104,8 +104,8 @@ variable_list backward_rows(const Tensor& x, const Tensor& g, const Tensor& weig
   const float* st = stats.const_data_ptr<float>();
   check(entries.bwd(xr.t.const_data_ptr(), xr.ld, gr.t.const_data_ptr(), gr.ld, type_code(x), w.data(), b.data(), st,
                     st + xr.count, xr.count, width, (int)act, need_x ? dx.mutable_data_ptr() : nullptr,
-                    need_cols ? dw.mutable_data_ptr<float>() : nullptr, need_cols ? db.mutable_data_ptr<float>() : nullptr,
-                    need_cols ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(x)),
+                    need_cols ? dw.mutable_data_ptr<float>() : nullptr,
+                    need_cols ? db.mutable_data_ptr<float>() : nullptr, need_cols ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(x)),
         "e2a_layer_norm_bwd");
   return {dx, dw, db};
 }
