@@ -398,7 +398,7 @@ int e2a_layer_norm_bwd2(const void* x, int64_t ldx, const void* dy, int64_t lddy
 /* Global norm: e2a_sum_squares writes partial sums (64 bits) of all values' squares to the          */
 /* workspace (e2a_grad_norm_workspace_bytes) and their number to the host; tensors of another type    */
 /* follow by further calls on the rest of the workspace.  e2a_norm_of_squares adds them up in order   */
-/* and writes the root.                                                                             */
+/* and writes the root.  e2a_grad_norm is both for tensors of one type.                              */
 /*                                                                                                  */
 /* e2a_adamw_step: per tensor j with t = ++step[slots[j]] (int32, device),                            */
 /*   g = grad min(1, max_norm / (grad_norm + 1e-6))   (grad_norm device fp32, or NULL: no clipping)   */
@@ -417,6 +417,8 @@ size_t e2a_grad_norm_workspace_bytes(int64_t n_tensors);
 int e2a_sum_squares(const uint64_t* tensors, const int64_t* numel, int64_t n_tensors, int dtype, void* workspace,
                     size_t workspace_bytes, int64_t* n_partials, void* stream);
 int e2a_norm_of_squares(const void* partials, int64_t n_partials, float* norm, void* stream);
+int e2a_grad_norm(const uint64_t* tensors, const int64_t* numel, int64_t n_tensors, int dtype, void* workspace,
+                  size_t workspace_bytes, float* norm, void* stream);
 size_t e2a_adamw_workspace_bytes(int64_t n_tensors);
 int e2a_adamw_step(const uint64_t* params, const uint64_t* grads, const int64_t* numel, const int64_t* state_offset,
                    const int32_t* slots, int64_t n_tensors, int dtype, int state_bits, void* exp_avg, void* exp_avg_sq,

@@ -179,6 +179,8 @@ def test_c_abi_refuses_bad_arguments():
     assert lib.e2a_sum_squares(t.buffer_info()[0], k.buffer_info()[0], 1, 0, dev, 0, n.buffer_info()[0], None) == 3
     assert lib.e2a_sum_squares(None, None, 0, 0, None, 0, n.buffer_info()[0], None) == 0 and n[0] == 0
     assert lib.e2a_norm_of_squares(None, 0, None, None) == 1 and lib.e2a_norm_of_squares(None, 4, dev, None) == 1
+    assert lib.e2a_grad_norm(t.buffer_info()[0], k.buffer_info()[0], 1, 0, dev, 0, dev, None) == 3
+    assert lib.e2a_grad_norm(t.buffer_info()[0], k.buffer_info()[0], -1, 0, dev, 64, dev, None) == 1
     assert lib.e2a_moments_unpack(None, None, None, None, 5, None, None, None) == 1
 
 

@@ -91,6 +91,7 @@ SIGNATURES = {
     "e2a_grad_norm_workspace_bytes": (SZ, [I64]),
     "e2a_sum_squares": (I32, [P, P, I64, I32, P, SZ, P, P]),
     "e2a_norm_of_squares": (I32, [P, I64, P, P]),
+    "e2a_grad_norm": (I32, [P, P, I64, I32, P, SZ, P, P]),
     "e2a_adamw_workspace_bytes": (SZ, [I64]),
     "e2a_adamw_step": (I32, [P, P, P, P, P, I64, I32, I32, P, P, P, P, I64, P, F64, P, F64, F64, F64, F64, P, F64,
                              P, SZ, P]),

@@ -677,6 +677,13 @@ int e2a_norm_of_squares(const void* partials, int64_t n_partials, float* norm, v
   return E2A_OK;
 }
 
+int e2a_grad_norm(const uint64_t* tensors, const int64_t* numel, int64_t n_tensors, int dtype, void* workspace,
+                  size_t workspace_bytes, float* norm, void* stream) {
+  int64_t n = 0;
+  const int rc = e2a_sum_squares(tensors, numel, n_tensors, dtype, workspace, workspace_bytes, &n, stream);
+  return rc == E2A_OK ? e2a_norm_of_squares(workspace, n, norm, stream) : rc;
+}
+
 size_t e2a_adamw_workspace_bytes(int64_t n_tensors) {
   return n_tensors <= 0 ? 0 : sizeof(Globals) + (size_t)n_tensors * sizeof(Scalars);
 }

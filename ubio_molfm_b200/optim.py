@@ -8,6 +8,7 @@ pipeline/trainer.py:397-414), so a training step can be captured in a CUDA graph
 from __future__ import annotations
 
 from array import array
+from contextlib import nullcontext
 from operator import attrgetter
 
 import torch
@@ -73,7 +74,13 @@ def _norm(dev, lists):
     norm = torch.empty((), dtype=torch.float32, device=dev)
     size = sum(lib.e2a_grad_norm_workspace_bytes(n) for _, n, _, _ in lists)
     ws = torch.empty(max(size, 8), dtype=torch.uint8, device=dev)
-    base, done, count = ws.data_ptr(), 0, array("q", (0,))
+    base = ws.data_ptr()
+    if len(lists) == 1:
+        (code, n, at, numel), = lists
+        check(lib.e2a_grad_norm(_address(at), _address(numel), n, code, base, size, norm.data_ptr(), stream),
+              "e2a_grad_norm")
+        return norm
+    done, count = 0, array("q", (0,))
     for code, n, at, numel in lists:
         check(lib.e2a_sum_squares(_address(at), _address(numel), n, code, base + 8 * done, size - 8 * done,
                                   _address(count), stream), "e2a_sum_squares")
@@ -96,9 +103,7 @@ def grad_norm(tensors):
         tensors = _contiguous(tensors)
         lists = [(code, len(ts), _pointers(ts), array("q", map(torch.Tensor.numel, ts)))
                  for code, ts in _by_type("grad_norm", tensors)]
-    if dev.index == torch.cuda.current_device():
-        return _norm(dev, lists)
-    with torch.cuda.device(dev):
+    with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else nullcontext():
         return _norm(dev, lists)
 
 
