@@ -15,7 +15,8 @@
 // are dropped after adding an offset, mixed bits of (element, step), so a value is rounded up as often as it is
 // near the upper neighbour: round-to-nearest would never move an average whose step is 1 - b2 = 1e-3 of itself
 // (an additive sequence in place of mixed bits locks to the value that it rounds: an average that grows by 1e-3
-// a step fell 6% behind in 2,000 steps).  sqrt(v) > 0 is never rounded to 0 (the update would divide by eps).
+// a step fell 6% behind in 2,000 steps).  sqrt(v) over 2^-63 is never rounded to 0 (the update
+// would divide by eps).
 // The moments' operations are single rounded fp32 ones in a fixed order, so the codes are reproducible bit for bit.
 //
 // With 32-bit moments it is bound by memory: 24.5M fp32 parameters in 240 tensors (28 bytes each) take 99 us, 6.9 TB/s.
