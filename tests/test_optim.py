@@ -150,6 +150,13 @@ def test_constructor_refusals():
         grad_norm([torch.ones(3)])
 
 
+def test_streams_are_of_cuda_devices():
+    from ubio_molfm_b200 import _lib
+
+    with pytest.raises((ValueError, RuntimeError, AssertionError)):      # no device to ask, or not one of CUDA's
+        _lib.stream_of(torch.device("cpu"))
+
+
 def test_c_abi_refuses_bad_arguments():
     """Every check comes before device work: the addresses are never read."""
     from ubio_molfm_b200 import _lib

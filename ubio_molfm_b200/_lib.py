@@ -204,10 +204,9 @@ def ptr(t):
 def stream_of(device) -> ctypes.c_void_p:
     """The current stream of ``device`` (None: of the current device).  The raw handle: building a
     ``torch.cuda.Stream`` around it costs as much as a launch."""
-    index = getattr(device, "index", device)
-    if not isinstance(index, int):
-        index = torch.cuda.current_device()
-    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))
+    if isinstance(device, torch.device) and device.type == "cuda" and device.index is not None:
+        return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))
+    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
 def require_cuda(*tensors):
