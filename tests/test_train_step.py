@@ -119,7 +119,7 @@ def test_train_step(bits):
 
 
 def test_train_step_runs_on_and_refuses_bad_targets():
-    from ubio_molfm_b200.interface import E2FormerModelInterface
+    from ubio_molfm_b200.interface import E2FormerModelInterface, collate_systems
     from ubio_molfm_b200.optim import AdamW
 
     batch = _molecules()
@@ -127,10 +127,13 @@ def test_train_step_runs_on_and_refuses_bad_targets():
     iface = E2FormerModelInterface(model=pot, device=DEV)
     opt = AdamW(pot.parameters(), lr=1e-4, state_bits=8, max_grad_norm=10.0)
     zero_e, zero_f = torch.zeros(4), torch.zeros_like(batch["pos"])
+    box = collate_systems([dict(atoms=_box()[1], coords=_box()[0], cell=_box()[2], pbc=[True] * 3)], device=DEV)
+    assert bool(torch.isfinite(iface.train_step(box, torch.zeros(1), torch.zeros_like(box["pos"]), opt)))    # periodic
     for _ in range(3):
         assert bool(torch.isfinite(iface.train_step(batch, zero_e, zero_f, opt)))
-    with pytest.raises(RuntimeError):
-        iface.train_step(batch, torch.zeros(3), zero_f, opt)
+    for bad_e, bad_f in ((torch.zeros(3), zero_f), (torch.zeros(1), zero_f), (zero_e, zero_f[:, :5]), (zero_e, zero_f[0])):
+        with pytest.raises(ValueError, match="targets"):
+            iface.train_step(batch, bad_e, bad_f, opt)
     assert not pot.training
     # targets that are not finite: the step is left out, weights and states stay
     held = [p.detach().clone() for p in pot.parameters()] + [t.clone() for t in opt.flat_state().values()]

@@ -164,11 +164,16 @@ class E2FormerModelInterface:
         mode = self.model.training
         mask = model_input["atom_masks"].to(self.device).bool()
         counts = mask.sum(-1).clamp(min=1)
+        energy = torch.as_tensor(energy, device=self.device).reshape(-1)
+        forces = torch.as_tensor(forces, device=self.device)
+        if energy.numel() != mask.shape[0] or forces.shape != (*mask.shape, 3):
+            raise ValueError(f"targets of a batch of {list(mask.shape)} atoms: energy [{mask.shape[0]}] and forces "
+                             f"{[*mask.shape, 3]}, got {list(energy.shape)} and {list(forces.shape)}")
         self.model.train()
         try:
             out = self.predict(model_input)
-            de = (out["pred_energy"] - torch.as_tensor(energy, device=self.device).reshape(-1)) / counts
-            df = (out["pred_forces"] - torch.as_tensor(forces, device=self.device))[mask]
+            de = (out["pred_energy"] - energy) / counts
+            df = (out["pred_forces"] - forces)[mask]
             loss = energy_weight * de.square().mean() + force_weight * df.square().sum(-1).mean()
             optimizer.zero_grad()
             with projection_precision("tf32" if self.use_tf32 else "fp32"):
