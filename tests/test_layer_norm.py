@@ -209,9 +209,15 @@ def test_layer_norm_and_gradients_to_second_order(rows, width, dtype, silu):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,width", [(40000, 16), (20011, 64), (70001, 128), (9001, 512), (3001, 771), (600, 8200)])
-def test_many_rows(rows, width):
-    x, w, b, g, u, p, q = _inputs(rows, width, torch.float32)
+@pytest.mark.parametrize("rows,width,dtype", [
+    (40000, 16, torch.float32), (20011, 64, torch.float32), (70001, 128, torch.float32), (9001, 512, torch.float32),
+    (3001, 771, torch.float32), (600, 8200, torch.float32), (150001, 3, torch.float16), (50001, 25, torch.bfloat16),
+    (50003, 26, torch.float16), (40001, 77, torch.bfloat16), (30007, 131, torch.float16), (20001, 250, torch.bfloat16),
+    (20011, 300, torch.float16), (9001, 771, torch.bfloat16), (5003, 1203, torch.float16), (3001, 3001, torch.bfloat16),
+    (1201, 4089, torch.float16), (1201, 4091, torch.bfloat16)])
+def test_many_rows(rows, width, dtype):
+    """More rows than the device holds at once, past the fp32 chains' length, at every way of reading them."""
+    x, w, b, g, u, p, q = _inputs(rows, width, dtype)
     ref, major = reference(x, w, b, True, g, u, p, q), _majorants(x, w, b, g, u, p, q)
     got = _run(x, w, b, True, g, (u, p, q))
     for k, t in got.items():
