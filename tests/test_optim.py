@@ -150,6 +150,34 @@ def test_constructor_refusals():
         grad_norm([torch.ones(3)])
 
 
+def unlike_gradients():
+    """Parameters whose gradients are not of their type, size or device, with the error each is to raise."""
+    def of(device, grad, data=None):
+        p = torch.nn.Parameter(torch.zeros(4, device=device))
+        if grad != torch.float32:
+            p.grad_dtype = grad
+        p.grad = torch.ones(4, dtype=grad, device=device)
+        if data is not None:
+            p.data = data
+        return p
+
+    return [(lambda dev: of(dev, torch.bfloat16), TypeError), (lambda dev: of(dev, torch.float64), TypeError),
+            (lambda dev: of(dev, torch.float32, torch.zeros(4, dtype=torch.bfloat16, device=dev)), TypeError),
+            (lambda dev: of(dev, torch.float32, torch.zeros(1000, device=dev)), ValueError),
+            (lambda dev: of(dev, torch.float32, torch.zeros(2, device=dev)), ValueError)]
+
+
+def test_unlike_gradients_are_refused_on_the_host():
+    from ubio_molfm_b200.optim import _gradients
+
+    for make, error in unlike_gradients():
+        with pytest.raises(error, match="gradient"):
+            _gradients([make("cpu")])
+    p = torch.nn.Parameter(torch.zeros(4, 2))
+    p.grad = torch.arange(8.0).reshape(2, 4).t()
+    assert torch.equal(_gradients([p])[0], p.grad) and _gradients([p])[0].is_contiguous()
+
+
 def test_streams_are_of_cuda_devices():
     from ubio_molfm_b200 import _lib
 
@@ -591,6 +619,23 @@ def test_sparse_gradients_are_refused():
         AdamW(e.parameters()).step()
     with pytest.raises(TypeError):
         grad_norm([e.weight.grad])
+
+
+@pytest.mark.gpu
+def test_unlike_gradients_are_refused():
+    from ubio_molfm_b200.optim import AdamW
+
+    for make, error in unlike_gradients():
+        for bits in (32, 8):
+            p, q = make(DEV), torch.nn.Parameter(torch.ones(5, device=DEV))
+            q.grad = torch.ones(5, device=DEV)
+            opt = AdamW([q, p], state_bits=bits, max_grad_norm=1.0)
+            with pytest.raises(error, match="gradient"):
+                opt.step()
+            assert (q == 1).all() and (p == 0).all() and not opt.flat_state()["step"].any()
+            p.grad = None
+            opt.step()
+            assert (q != 1).all() and opt.flat_state()["step"].tolist() == [1, 0]
 
 
 @pytest.mark.gpu

@@ -59,6 +59,18 @@ def _contiguous(tensors):
     return [t.detach().contiguous() for t in tensors]
 
 
+def _gradients(params):
+    """The parameters' gradients, contiguous.  A gradient can differ from its parameter in type (``grad_dtype``) or,
+    after ``p.data = ...``, in size and device; the kernels read both alike."""
+    for p in params:
+        if p.grad.dtype != p.dtype:
+            raise TypeError(f"a {p.dtype} parameter has a {p.grad.dtype} gradient")
+        if p.grad.numel() != p.numel() or p.grad.device != p.device:
+            raise ValueError(f"a parameter of {p.numel()} values on {p.device} has a gradient of {p.grad.numel()} on "
+                             f"{p.grad.device}")
+    return _contiguous([p.grad for p in params])
+
+
 def _by_type(what, tensors, *others):
     """``[(type code, tensors, *others)]``: the lists split by the tensors' types."""
     kinds = set(map(_dtype, tensors))
@@ -311,7 +323,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW takes contiguous parameters")
         if any(p.numel() != flat.numel[k] for k, p in zip(index, params)):
             raise ValueError("a parameter has changed its size since its state was made")
-        grads = _contiguous([p.grad for p in params])
+        grads = _gradients(params)
         keep.append(grads)
         work = [(group, flat, code, len(ps), _pointers(ps), _pointers(gs), *(
             array(a.typecode, [a[k] for k in ks]) for a in (flat.numel, flat.offset, flat.slot)))
