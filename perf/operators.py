@@ -155,9 +155,8 @@ def prepare(case, seed):
         index = (torch.arange(total, device=DEV) - torch.repeat_interleave(
             torch.tensor(offsets, device=DEV), reps, output_size=total)).view(-1, BLOCK)
         st["index"] = index
-        dm, dv = _dither(index, st["step"][:1])
-        st["m"], st["ms"] = _pack(m.view(-1, BLOCK), dm, 3)
-        st["v"], st["vs"] = _pack(v.sqrt().view(-1, BLOCK), dv, 4)
+        st["m"], st["ms"] = _pack(m.view(-1, BLOCK), _dither(index, st["step"][:1], 0), 3)
+        st["v"], st["vs"] = _pack(v.sqrt().view(-1, BLOCK), _dither(index, st["step"][:1], 1), 4)
     else:
         st["m"], st["v"] = m, v
     if own:
@@ -181,27 +180,24 @@ def prepare(case, seed):
 
 # ------------------------------------------------------------------------------------------------
 # 8-bit moments, in elementary operations.  A block of 256 values shares the power of two of its largest
-# magnitude (the next one where rounding up could pass the largest code); a value over it is a small float of
-# 4 exponent bits and 3 (signed first moment) or 4 (square root of the second moment) fraction bits, rounded up
-# where mixed bits of (element, step) say so.
+# magnitude; a value over it is a small float of 4 exponent bits and 3 (signed first moment) or 4 (square
+# root of the second moment) fraction bits, rounded up with the probability that a fixed sequence over
+# elements and steps gives.
 # ------------------------------------------------------------------------------------------------
-# odd 32-bit fractions of the powers of the root of x^5 = x + 1
-_MIX = (0xDB4F0B91, 0xBBE05633, 0xA0F2EC75, 0x89E18285)
+# odd 32-bit fractions of the powers of the root of x^5 = x + 1: additive sequences with independent steps
+_INDEX_STEP = (0xDB4F0B91, 0xA0F2EC75)
+_TIME_STEP = (0xBBE05633, 0x89E18285)
 
 
-def _dither(index, step):
-    """Mixed bits of (element, step), uniform: the offsets of the first moment (below 2^20) and of the second
-    (below 2^19), [blocks, 256]."""
-    u = (index * _MIX[0] + step.long() * _MIX[1]) & 0xFFFFFFFF
-    u = ((u ^ (u >> 16)) * _MIX[2]) & 0xFFFFFFFF
-    u = ((u ^ (u >> 15)) * _MIX[3]) & 0xFFFFFFFF
-    u = u ^ (u >> 16)
-    return (u >> 12).int(), (u & 0x7FFFF).int()
+def _dither(index, step, which):
+    """Uniform values below 2^20 (first moment) or 2^19 (second), [blocks, 256]."""
+    u = (index * _INDEX_STEP[which] + step.long() * _TIME_STEP[which]) & 0xFFFFFFFF
+    return (u >> (12 + which)).int()
 
 
 def _pack(x, dither, fraction):
     mag = x.abs()
-    b = ((mag.amax(1, keepdim=True).view(torch.int32) + (1 << (23 - fraction))) >> 23).clamp(27, 253)
+    b = (mag.amax(1, keepdim=True).view(torch.int32) >> 23).clamp(27, 253)
     z = mag * ((254 - b) << 23).view(torch.float32) * 2.0 ** -112
     top = 127 if fraction == 3 else 255
     code = ((z.view(torch.int32) + dither) >> (23 - fraction)).clamp(max=top)
@@ -339,9 +335,8 @@ def _run_adamw(st):
         new = p * (1 - LR * DECAY) - m / (v.sqrt() * root + ADAM_EPS) * size
         st["p"].copy_(new.view(-1))
         if case["bits"] == 8:
-            dm, dv = _dither(st["index"], st["step"][:1])
-            st["m"], st["ms"] = _pack(m, dm, 3)
-            st["v"], st["vs"] = _pack(v.sqrt(), dv, 4)
+            st["m"], st["ms"] = _pack(m, _dither(st["index"], st["step"][:1], 0), 3)
+            st["v"], st["vs"] = _pack(v.sqrt(), _dither(st["index"], st["step"][:1], 1), 4)
             m, s = _unpack(st["m"], st["ms"], 3), _unpack(st["v"], st["vs"], 4)
             v = s * s
         else:
