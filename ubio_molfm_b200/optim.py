@@ -155,7 +155,9 @@ class AdamW(torch.optim.Optimizer):
     float16, contiguous, the arithmetic in fp32 with one rounding to the parameter's type.
 
     * ``state_bits``: 32 = fp32 moments; 8 = one byte per element and moment plus one scale byte per 256
-      (see ``csrc/e2a_optim.cu``), rounded so that averages stay unbiased over steps.
+      (see ``csrc/e2a_optim.cu``).  An 8-bit value is rounded either way as often as it is near, but what passes a
+      block's largest code stays there: random gradients leave sqrt(v) 1.4% low in the mean and the largest of each
+      256 about 40%, gradients that never change leave it at 1/8 to 1/4 of its value (steps up to 8 times as long).
     * ``max_grad_norm``: clip the gradients of each step to this global norm (over all groups) inside the update;
       the gradients themselves are left as they are.  The norm of the last step is ``last_grad_norm`` (0-dim
       tensor on the device).  A step whose norm is not finite changes nothing, step counts included.
