@@ -265,3 +265,33 @@ def test_late_steps_wrap_the_sequences():
     opt.step()
     _, m, v = step32(z, _np(p.grad), z, z, 2 ** 31 - 2, 1e-3, 0.9, 0.999, 1e-8, 1e-2)
     _check_state(opt.state[p], m, v, 2 ** 31 - 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eps", [0.0, 1e-8])
+def test_second_moments_below_the_normal_range(eps):
+    """Gradients of order 1 beside ones whose squares are subnormal, in whole blocks and in one that is cut short: a
+    second moment over 0 keeps a root over 0, and with eps = 0 the update has it in its denominator."""
+    from ubio_molfm_b200.optim import AdamW
+
+    n = 4 * 256 + 99
+    rng = np.random.default_rng(8)
+    g = rng.normal(size=n)
+    tiny = rng.random(n) < 0.5
+    g[tiny] = rng.choice([-1, 1], tiny.sum()) * np.exp(rng.uniform(np.log(4e-21), np.log(2e-17), tiny.sum()))
+    g[300:400] = 0
+    g = g.astype(F)
+    p0 = rng.normal(size=n).astype(F)
+    if eps == 0:
+        g[300:400] = 1.0                         # 0 / 0 is not a number, here as in the formula
+    p = torch.nn.Parameter(torch.from_numpy(p0.copy()).to(DEV))
+    p.grad = torch.from_numpy(g).to(DEV)
+    opt = AdamW([p], lr=1e-2, betas=(0.9, 0.999), eps=eps, weight_decay=0.0, state_bits=8)
+    r = dict(p=p0, m=np.zeros(n, F), v=np.zeros(n, F))
+    for t in (1, 2, 3):
+        opt.step()
+        new, m, v = step32(r["p"], g, r["m"], r["v"], t, 1e-2, 0.9, 0.999, eps, 0.0)
+        assert ((v > 0) == (g != 0)).all() and np.isfinite(new).all()
+        assert _same_p(_np(p), r["p"], new, torch.float32), t
+        r["p"] = _np(p)
+        r["m"], r["v"] = _check_state(opt.state[p], m, v, t)

@@ -303,11 +303,10 @@ __device__ __forceinline__ Codes block_fast(const Codes& h, T* pt, const T* gt, 
   for (int half = 0; half < 2; ++half) {
     float4 p4 = load4(pt, w.i + 128 * half, w.n, vec);
     const float4 g4 = load4(gt, w.i + 128 * half, w.n, vec);
+    float2 v[2];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int e = 2 * half + q;
       float2 g = q ? make_float2(g4.z, g4.w) : make_float2(g4.x, g4.y);
-      const float2 p = q ? make_float2(p4.z, p4.w) : make_float2(p4.x, p4.y);
       if (clip) g = f2_mul(g, f2(gl.coef));
       const uint32_t a0 = byte_on_top(h.m[half], 2 * q), a1 = byte_on_top(h.m[half], 2 * q + 1);
       const uint32_t b0 = byte_on_top(h.s[half], 2 * q) >> 5, b1 = byte_on_top(h.s[half], 2 * q + 1) >> 5;
@@ -315,9 +314,20 @@ __device__ __forceinline__ Codes block_fast(const Codes& h, T* pt, const T* gt, 
       const float2 m0 = f2_mul(make_float2(__uint_as_float((uint32_t)((int32_t)a0 >> 4) & 0x87F00000u),
                                            __uint_as_float((uint32_t)((int32_t)a1 >> 4) & 0x87F00000u)), fm);
       const float2 s0 = f2_mul(make_float2(__uint_as_float(b0), __uint_as_float(b1)), fs);
-      m[e] = sum_of_products(m0, r.b1, g, r.a1, r.one);
-      const float2 v = sum_of_products(f2_mul(s0, s0), r.b2, f2_mul(g, g), r.a2, r.one);
-      s[e] = make_float2(root_approx(v.x), root_approx(v.y));
+      m[2 * half + q] = sum_of_products(m0, r.b1, g, r.a1, r.one);
+      v[q] = sum_of_products(f2_mul(s0, s0), r.b2, f2_mul(g, g), r.a2, r.one);
+      s[2 * half + q] = make_float2(root_approx(v[q].x), root_approx(v[q].y));
+    }
+    // a second moment over 0 but below 2^-126, whose root is not 0 (a 0's bits less 1 are the largest)
+    if (min(min(__float_as_uint(v[0].x) - 1u, __float_as_uint(v[0].y) - 1u),
+            min(__float_as_uint(v[1].x) - 1u, __float_as_uint(v[1].y) - 1u)) < 0x007FFFFFu) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) s[2 * half + q] = make_float2(__fsqrt_rn(v[q].x), __fsqrt_rn(v[q].y));
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int e = 2 * half + q;
+      const float2 p = q ? make_float2(p4.z, p4.w) : make_float2(p4.x, p4.y);
       const float2 d = f2_fma(s[e], f2(sc.root), f2(r.eps));
       const float2 up = f2_mul(m[e], make_float2(reciprocal(d.x), reciprocal(d.y)));
       const float2 next = f2_fma(up, f2(-sc.size), f2_mul(p, f2(gl.decay)));
@@ -355,8 +365,8 @@ __device__ __forceinline__ Codes block_fast(const Codes& h, T* pt, const T* gt, 
         const uint32_t at = 2 * q + k + 128 * half;
         const uint32_t tm = __float_as_uint(__fmul_rn(fabsf(me[k]), zm)) + ((w.um + at * kIndexStepM) >> 12);
         cm[2 * q + k] = (min(tm, 0x07FFFFFFu) << 4) | (__float_as_uint(me[k]) & 0x80000000u);
-        // over zero at least the smallest code (a root of a subnormal, 0 here, counts as zero); 4 more than the
-        // sum, so that what is in doubt lies in 0..7 of the dropped bits
+        // over zero at least the smallest code; 4 more than the sum, so that what is in doubt lies in 0..7 of the
+        // dropped bits
         const float least = fminf(se[k], __uint_as_float(1u << 19));
         const uint32_t ts = __float_as_uint(fmaxf(ze[k], least)) + ((w.us + at * kIndexStepS) >> 13) + 4u;
         doubt = min(doubt, ts & 0x7FFFFu);
