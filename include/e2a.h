@@ -404,9 +404,10 @@ int e2a_layer_norm_bwd2(const void* x, int64_t ldx, const void* dy, int64_t lddy
 /*   g = grad min(1, max_norm / (grad_norm + 1e-6))   (grad_norm device fp32, or NULL: no clipping)   */
 /*   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2                                      */
 /*   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)         */
-/* in fp32, p rounded once to its type.  Unless *grad_norm is finite nothing is changed, step          */
-/* included.  lr_device (fp32, may be NULL) takes lr's place.  The moments are flat: tensor j's start   */
-/* at element state_offset[j], a multiple of 256, in order; slots rise too.  state_bits 32: fp32.      */
+/* in fp32, p rounded once to its type; eps is 0 or at least 2^-126 (its reciprocal is an fp32 one).    */
+/* Unless *grad_norm is finite nothing is changed, step included.  lr_device (fp32, may be NULL) takes   */
+/* lr's place.  The moments are flat: tensor j's start at element state_offset[j], a multiple of 256,     */
+/* in order; slots rise too.  state_bits 32: fp32.                                                     */
 /* state_bits 8: one byte an element and, per 256 of them, one scale byte: x = y 2^(scale - 127) with   */
 /* y a small float, m: sign, 4 exponent, 3 fraction bits; sqrt(v): 4 exponent, 4 fraction bits; exponent */
 /* 15 stands for [1, 2), 0 for the subnormals; scale 255 for a block of NaN.  e2a_moments_unpack gives   */

@@ -702,6 +702,7 @@ int e2a_adamw_step(const uint64_t* params, const uint64_t* grads, const int64_t*
   if (bad_tensors(params, numel, n_tensors, dtype) || bad_tensors(grads, numel, n_tensors, dtype)) return E2A_ERR_ARG;
   if (state_bits != 32 && state_bits != 8) return E2A_ERR_ARG;
   if (!(beta1 >= 0. && beta1 < 1. && beta2 >= 0. && beta2 < 1. && eps >= 0.)) return E2A_ERR_ARG;
+  if (eps > 0. && eps < 0x1p-126) return E2A_ERR_ARG;      // the kernels' reciprocal takes it for 0
   if (grad_norm && !(max_norm > 0.)) return E2A_ERR_ARG;
   if (n_tensors == 0) return E2A_OK;
   if (!state_offset || !slots || !exp_avg || !exp_avg_sq || !step || n_tensors > (1 << 24)) return E2A_ERR_ARG;

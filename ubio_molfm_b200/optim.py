@@ -152,7 +152,8 @@ class _Flat:
 
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) with PyTorch's arguments and update; parameters in float32, bfloat16 or
-    float16, contiguous, the arithmetic in fp32 with one rounding to the parameter's type.
+    float16, contiguous, the arithmetic in fp32 with one rounding to the parameter's type; ``eps`` is 0 or at least
+    2^-126.
 
     * ``state_bits``: 32 = fp32 moments; 8 = one byte per element and moment plus one scale byte per 256
       (see ``csrc/e2a_optim.cu``).  An 8-bit value is rounded either way as often as it is near, but what passes a
@@ -185,6 +186,8 @@ class AdamW(torch.optim.Optimizer):
             b1, b2 = g["betas"]
             if not (0 <= b1 < 1 and 0 <= b2 < 1 and g["eps"] >= 0 and g["weight_decay"] >= 0):
                 raise ValueError(f"invalid betas {g['betas']}, eps {g['eps']} or weight_decay {g['weight_decay']}")
+            if 0 < g["eps"] < 2.0 ** -126:
+                raise ValueError(f"eps={g['eps']} is below the normal fp32 range: 0, or at least 2^-126")
             if not isinstance(g["lr"], torch.Tensor) and not g["lr"] >= 0:
                 raise ValueError(f"invalid lr {g['lr']}")
             if len(set(map(id, g["params"]))) != len(g["params"]):
