@@ -146,7 +146,9 @@ def load_torch():
         lib.e2a_tensor_table.restype = I32
         lib.e2a_tensor_table.argtypes = [ctypes.py_object, I64, P, P, P, P]
         lib.e2a_step_table.restype = I32
-        lib.e2a_step_table.argtypes = [ctypes.py_object, I64, P, P, P, P, P, P, P, P, P, P]
+        lib.e2a_step_table.argtypes = [ctypes.py_object, ctypes.py_object, I64, P, P, P]
+        lib.e2a_state_is_held.restype = I32
+        lib.e2a_state_is_held.argtypes = [ctypes.py_object, ctypes.py_object, I64]
         lib.e2a_layer_norm.restype = ctypes.py_object
         lib.e2a_layer_norm.argtypes = [ctypes.py_object, ctypes.py_object, ctypes.py_object, F64, I32]
         lib.e2a_torch_bind.restype = None

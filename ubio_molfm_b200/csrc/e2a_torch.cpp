@@ -270,37 +270,55 @@ __attribute__((visibility("default"))) int e2a_tensor_table(PyObject* tensors, i
   }
 }
 
-// The optimiser's table of a list of n parameters: for the *count of them that have a gradient, in order, the
-// addresses of both, their number of elements (that of held_numel, or 1 is returned), their held_offset and their
-// place in the list; counts a new version of each, since the kernels write behind autograd's back.  Returns as
-// above, with *count 0 and no type where no parameter has a gradient.
-__attribute__((visibility("default"))) int e2a_step_table(PyObject* params, int64_t n, const int64_t* held_numel,
-                                                          const int64_t* held_offset, uint64_t* address,
-                                                          uint64_t* grads, int64_t* numel, int64_t* offset,
-                                                          int32_t* slot, int32_t* type, int32_t* device,
-                                                          int32_t* count) {
+// Whether a dict of dicts, an optimiser's state, is as it was noted: `held` is the list of n objects (key, entry, tuple
+// of the entry's values) of every item, in the dict's order.  Compared by identity; returns 0 where all are the same.
+__attribute__((visibility("default"))) int e2a_state_is_held(PyObject* state, PyObject* held, int64_t n) {
+  if (!PyDict_Check(state) || !PyList_CheckExact(held) || PyList_GET_SIZE(held) != n) return 1;
+  PyObject *key, *entry, *value;
+  int64_t i = 0;
+  for (Py_ssize_t at = 0; PyDict_Next(state, &at, &key, &entry); i += 3) {
+    if (i + 3 > n || PyList_GET_ITEM(held, i) != key || PyList_GET_ITEM(held, i + 1) != entry) return 1;
+    PyObject* values = PyList_GET_ITEM(held, i + 2);
+    if (!PyDict_Check(entry) || !PyTuple_CheckExact(values)) return 1;
+    Py_ssize_t k = 0;
+    for (Py_ssize_t in = 0; PyDict_Next(entry, &in, nullptr, &value); ++k)
+      if (k >= PyTuple_GET_SIZE(values) || PyTuple_GET_ITEM(values, k) != value) return 1;
+    if (k != PyTuple_GET_SIZE(values)) return 1;
+  }
+  return i == n ? 0 : 1;
+}
+
+// The optimiser's table of a list of n parameters, which have to be those of the list `held`: for those that have a
+// gradient, in order, the addresses of both, their number of elements (that of held_numel, or 1 is returned), their
+// held_offset and their place in the list (int32), each from a multiple of n on in `table`; behind 5 n, type << 32 |
+// device and their number.  Counts a new version of each, since the kernels write behind autograd's back.  Returns as
+// above, with the number 0 and no type where no parameter has a gradient.
+__attribute__((visibility("default"))) int e2a_step_table(PyObject* params, PyObject* held, int64_t n,
+                                                          const int64_t* held_numel, const int64_t* held_offset,
+                                                          int64_t* table) {
   try {
     if (!PyList_CheckExact(params) || PyList_GET_SIZE(params) != n) return 1;
+    if (!PyList_CheckExact(held) || PyList_GET_SIZE(held) != n) return 1;
+    int32_t* slot = reinterpret_cast<int32_t*>(table + 4 * n);
     Common all;
-    int32_t k = 0;
+    int64_t k = 0;
     for (int64_t j = 0; j < n; ++j) {
       PyObject* o = PyList_GET_ITEM(params, j);
-      if (!THPVariable_Check(o)) return 1;
+      if (o != PyList_GET_ITEM(held, j) || !THPVariable_Check(o)) return 1;
       const Tensor& t = THPVariable_Unpack(o);
       const Tensor& g = t.grad();
       if (!g.defined()) continue;
       if (!all.take(t) || !all.take(g) || t.numel() != held_numel[j] || g.numel() != held_numel[j]) return 1;
-      address[k] = reinterpret_cast<uint64_t>(t.data_ptr());
-      grads[k] = reinterpret_cast<uint64_t>(g.data_ptr());
-      numel[k] = held_numel[j];
-      offset[k] = held_offset[j];
+      table[k] = reinterpret_cast<int64_t>(t.data_ptr());
+      table[n + k] = reinterpret_cast<int64_t>(g.data_ptr());
+      table[2 * n + k] = held_numel[j];
+      table[3 * n + k] = held_offset[j];
       slot[k++] = (int32_t)j;
     }
-    for (int32_t i = 0; i < k; ++i)
+    for (int64_t i = 0; i < k; ++i)
       torch::autograd::impl::bump_version(THPVariable_Unpack(PyList_GET_ITEM(params, slot[i])));
-    *type = all.type;
-    *device = all.device;
-    *count = k;
+    table[5 * n] = k ? (int64_t)all.type << 32 | all.device : 0;
+    table[5 * n + 1] = k;
     return 0;
   } catch (...) {
     return 1;

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 from array import array
 from contextlib import nullcontext
-from operator import attrgetter
+from operator import attrgetter, is_
 
 import torch
 
@@ -81,7 +81,8 @@ def _by_type(what, tensors, *others):
 
 
 def _norm(dev, lists):
-    """The norm of ``lists`` = [(type code, number, addresses, sizes)] of contiguous tensors on the current device."""
+    """The norm of ``lists`` = [(type code, number, where the tensors' addresses and sizes stand)] of contiguous tensors
+    on the current device."""
     lib, stream = _lib.load(), stream_of(dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     size = sum(lib.e2a_grad_norm_workspace_bytes(n) for _, n, _, _ in lists)
@@ -89,12 +90,12 @@ def _norm(dev, lists):
     base = ws.data_ptr()
     if len(lists) == 1:
         (code, n, at, numel), = lists
-        check(lib.e2a_grad_norm(_address(at), _address(numel), n, code, base, size, norm.data_ptr(), stream),
+        check(lib.e2a_grad_norm(at, numel, n, code, base, size, norm.data_ptr(), stream),
               "e2a_grad_norm")
         return norm
     done, count = 0, array("q", (0,))
     for code, n, at, numel in lists:
-        check(lib.e2a_sum_squares(_address(at), _address(numel), n, code, base + 8 * done, size - 8 * done,
+        check(lib.e2a_sum_squares(at, numel, n, code, base + 8 * done, size - 8 * done,
                                   _address(count), stream), "e2a_sum_squares")
         done += count[0]
     check(lib.e2a_norm_of_squares(base, done, norm.data_ptr(), stream), "e2a_norm_of_squares")
@@ -109,14 +110,14 @@ def grad_norm(tensors):
     found = _table(tensors) if tensors else None
     if found is not None:
         at, numel, code, index = found
-        dev, lists = torch.device("cuda", index), [(code, len(at), at, numel)]
+        dev, tables = torch.device("cuda", index), [(code, len(at), at, numel)]
     else:
         dev = _one_device(tensors, "the tensors") if tensors else torch.device("cuda", torch.cuda.current_device())
         tensors = _contiguous(tensors)
-        lists = [(code, len(ts), _pointers(ts), array("q", map(torch.Tensor.numel, ts)))
-                 for code, ts in _by_type("grad_norm", tensors)]
+        tables = [(code, len(ts), _pointers(ts), array("q", map(torch.Tensor.numel, ts)))
+                  for code, ts in _by_type("grad_norm", tensors)]
     with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else nullcontext():
-        return _norm(dev, lists)
+        return _norm(dev, [(code, n, _address(at), _address(numel)) for code, n, at, numel in tables])
 
 
 class _Flat:
@@ -124,12 +125,13 @@ class _Flat:
     count per tensor."""
 
     def __init__(self, params, bits):
-        self.device = _one_device(params, "a group's parameters")
+        self.device, self.params = _one_device(params, "a group's parameters"), list(params)
         self.numel, self.offset, end = array("q", map(torch.Tensor.numel, params)), array("q"), 0
         for n in self.numel:
             self.offset.append(end)
             end += -(-n // BLOCK) * BLOCK
         self.slot = array("i", range(len(params)))
+        self.at = _address(self.numel), _address(self.offset)
         self.elements, self.bits = end, bits
         kind = torch.float32 if bits == 32 else torch.uint8
         self.buffers = {"step": torch.zeros(len(params), dtype=torch.int32, device=self.device),
@@ -138,6 +140,8 @@ class _Flat:
         if bits == 8:
             for k in ("exp_avg_scale", "exp_avg_sq_scale"):
                 self.buffers[k] = torch.zeros(end // BLOCK, dtype=torch.uint8, device=self.device)
+        self.entries = [self.view(i, p) for i, p in enumerate(self.params)]
+        self.values = [tuple(e.values()) for e in self.entries]
 
     def view(self, i, param):
         """The state of tensor ``i``: views of the flat buffers."""
@@ -148,6 +152,24 @@ class _Flat:
             if k in self.buffers:
                 out[k] = self.buffers[k][o // BLOCK:(o + n + BLOCK - 1) // BLOCK]
         return out
+
+    def belongs_to(self, params):
+        return len(params) == len(self.params) and all(map(is_, params, self.params))
+
+    def held_in(self, state):
+        """Whether an optimiser's ``state`` has this state's views, and nothing else, for its parameters."""
+        return all(state.get(p) is e and len(e) == len(v) and all(map(is_, e.values(), v))
+                   for p, e, v in zip(self.params, self.entries, self.values))
+
+    def take(self, i, entry):
+        """Copies a state of tensor ``i`` from elsewhere."""
+        mine = self.entries[i]
+        if set(entry) != set(mine) or any(t.shape != mine[k].shape or (t.dtype != mine[k].dtype and k != "step")
+                                          for k, t in entry.items()):
+            raise ValueError(f"the state of a parameter of shape {list(self.params[i].shape)} is not one of "
+                             f"{self.bits}-bit moments")
+        for k, t in entry.items():
+            mine[k].copy_(t)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -167,7 +189,9 @@ class AdamW(torch.optim.Optimizer):
 
     Parameters without a gradient are left out of a step, each has its own step count.  State entries
     (``step``, ``exp_avg``, ``exp_avg_sq`` and, in 8 bits, their ``_scale``) are views of one flat buffer per
-    group (:meth:`flat_state`); ``state_dict`` / ``load_state_dict`` keep types and bits."""
+    group (:meth:`flat_state`); ``state_dict`` / ``load_state_dict`` keep types and bits.  As with PyTorch's, the
+    state belongs to the parameter: one that replaces another, or whose entry in ``state`` was cleared, starts anew,
+    and groups may be reordered, shortened or removed between steps (the next step then lays their state out again)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
                  max_grad_norm=None):
@@ -176,7 +200,7 @@ class AdamW(torch.optim.Optimizer):
         if max_grad_norm is not None and not max_grad_norm > 0:
             raise ValueError(f"max_grad_norm={max_grad_norm!r} must be positive")
         self.state_bits, self.max_grad_norm, self.last_grad_norm = state_bits, max_grad_norm, None
-        self._flat = {}
+        self._flat, self._held = {}, []
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, param_group):
@@ -197,13 +221,34 @@ class AdamW(torch.optim.Optimizer):
             raise
 
     # -- state -------------------------------------------------------------------------------------
+    def _sync(self):
+        """Drops the layouts that ``state`` no longer is the views of, whoever changed it; what it holds is laid out
+        again where a group needs it."""
+        if _lib.load_torch().e2a_state_is_held(self.state, self._held, len(self._held)):
+            self._flat = {i: f for i, f in self._flat.items() if i < len(self.param_groups) and f.held_in(self.state)}
+            self._hold()
+
+    def _hold(self):
+        """Notes ``state`` as it is: its keys, entries and their values."""
+        self._held = [x for p, e in self.state.items()
+                      for x in (p, e, tuple(e.values()) if isinstance(e, dict) else ())]
+
     def _group_state(self, i):
-        flat = self._flat.get(i)
-        if flat is None:
-            params = self.param_groups[i]["params"]
-            flat = self._flat[i] = _Flat(params, self.state_bits)
+        self._sync()
+        flat, params = self._flat.get(i), self.param_groups[i]["params"]
+        return flat if flat is not None and flat.belongs_to(params) else self._lay_out(i)
+
+    def _lay_out(self, i):
+        """A flat state for group ``i``, with what ``state`` has for its parameters and zeros for the others."""
+        params = self.param_groups[i]["params"]
+        flat = _Flat(params, self.state_bits)
+        with torch.no_grad():
             for k, p in enumerate(params):
-                self.state[p] = flat.view(k, p)
+                if self.state.get(p):
+                    flat.take(k, self.state[p])
+        self.state.update(zip(params, flat.entries))
+        self._flat[i] = flat
+        self._hold()
         return flat
 
     def flat_state(self, group=0):
@@ -241,15 +286,10 @@ class AdamW(torch.optim.Optimizer):
             if i in held and (held[i]["exp_avg"].shape != p.shape or held[i]["exp_avg_sq"].shape != p.shape):
                 raise ValueError(f"state of parameter {i} has another shape than the parameter")
         super().load_state_dict({"state": {}, "param_groups": groups})    # checks and takes the groups
-        self._flat = {}
-        with torch.no_grad():
-            for gi, (g, mine) in enumerate(zip(groups, self.param_groups)):
-                if not any(i in held for i in g["params"]):
-                    continue
-                self._group_state(gi)
-                for i, p in zip(g["params"], mine["params"]):
-                    for key, t in held.get(i, {}).items():
-                        self.state[p][key].copy_(t)
+        for gi, (g, mine) in enumerate(zip(groups, self.param_groups)):
+            if any(i in held for i in g["params"]):
+                self.state.update((p, held[i]) for i, p in zip(g["params"], mine["params"]) if i in held)
+                self._lay_out(gi)
 
     def __getstate__(self):
         return {**super().__getstate__(), "state_bits": self.state_bits, "max_grad_norm": self.max_grad_norm,
@@ -257,14 +297,10 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        held, self._flat = self.state, {}
+        self._flat, self._held = {}, []
         for gi, g in enumerate(self.param_groups):      # a copy's state becomes views of its own flat buffers
-            old = {k: held[p] for k, p in enumerate(g["params"]) if p in held}
-            if old:
-                self._group_state(gi)
-                for k, entries in old.items():
-                    for key, t in entries.items():
-                        self.state[g["params"][k]][key].copy_(t)
+            if any(self.state.get(p) for p in g["params"]):
+                self._lay_out(gi)
 
     # -- the step ----------------------------------------------------------------------------------
     @torch.no_grad()
@@ -273,6 +309,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        self._sync()
         work, keep = [], []
         for gi, g in enumerate(self.param_groups):
             work += self._group_work(gi, g, keep)
@@ -294,8 +331,9 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _group_work(self, gi, group, keep):
-        """The launches of a group: ``[(group, flat state, type code, number of tensors, addresses of the parameters
-        and of their gradients, sizes, state offsets, slots)]``; ``keep`` holds what has to live until then."""
+        """The launches of a group: ``[(group, flat state, type code, number of tensors, and where the addresses of the
+        parameters and of their gradients, their sizes, state offsets and slots stand)]``; ``keep`` holds what has to
+        live until then."""
         params = group["params"]
         if not params:
             return []
@@ -303,21 +341,13 @@ class AdamW(torch.optim.Optimizer):
         if flat is None:
             if all(p.grad is None for p in params):
                 return []
-            flat = self._group_state(gi)
-        n = len(params)
-        at, grads, numel, offset, slot = (_zeros(t, n) for t in "QQqqi")
-        info = _zeros("i", 3)
-        if n == len(flat.numel) and not _lib.load_torch().e2a_step_table(
-                params, n, _address(flat.numel), _address(flat.offset), _address(at), _address(grads), _address(numel),
-                _address(offset), _address(slot), _address(info), _address(info) + 4, _address(info) + 8):
-            code, index, count = info
-            if count == 0:
-                return []
-            if index != flat.device.index:
-                raise ValueError("the parameters have moved to another device than their state")
-            return [(group, flat, code, count, at, grads, numel, offset, slot)]
-        if n != len(flat.numel):
-            raise ValueError("the group's parameters are not those its state was made for")
+            flat = self._lay_out(gi)
+        found = self._read(group, flat, keep)
+        if found is None and not flat.belongs_to(params):
+            flat = self._lay_out(gi)
+            found = self._read(group, flat, keep)
+        if found is not None:
+            return found
         index = [k for k, p in enumerate(params) if p.grad is not None]
         if not index:
             return []
@@ -329,13 +359,31 @@ class AdamW(torch.optim.Optimizer):
         if any(p.numel() != flat.numel[k] for k, p in zip(index, params)):
             raise ValueError("a parameter has changed its size since its state was made")
         grads = _gradients(params)
-        keep.append(grads)
-        work = [(group, flat, code, len(ps), _pointers(ps), _pointers(gs), *(
-            array(a.typecode, [a[k] for k in ks]) for a in (flat.numel, flat.offset, flat.slot)))
-            for code, ps, gs, ks in _by_type("AdamW", params, grads, index)]
+        work = []
+        for code, ps, gs, ks in _by_type("AdamW", params, grads, index):
+            table = [_pointers(ps), _pointers(gs), *(array(a.typecode, [a[k] for k in ks])
+                                                     for a in (flat.numel, flat.offset, flat.slot))]
+            keep.append((grads, table))
+            work.append((group, flat, code, len(ps), *map(_address, table)))
         # the kernels write behind autograd's back: saved tensors and caches keyed on versions have to see it
         torch.autograd.graph.increment_version(params)
         return work
+
+    @staticmethod
+    def _read(group, flat, keep):
+        """The launch of a group whose parameters are those of ``flat`` and all alike, in one call; else None."""
+        params, n = group["params"], len(flat.params)
+        table = _zeros("q", 5 * n + 2)
+        at = _address(table)
+        if len(params) != n or _lib.load_torch().e2a_step_table(params, flat.params, n, flat.at[0], flat.at[1], at):
+            return None
+        two, count = divmod(table[5 * n], 1 << 32), table[5 * n + 1]
+        if count == 0:
+            return []
+        if two[1] != flat.device.index:
+            raise ValueError("the parameters have moved to another device than their state")
+        keep.append(table)
+        return [(group, flat, two[0], count, at, at + 8 * n, at + 16 * n, at + 24 * n, at + 32 * n)]
 
     def _launch(self, group, flat, code, count, at, grads, numel, offset, slot, norm):
         lr, lr_at = group["lr"], None
@@ -351,7 +399,6 @@ class AdamW(torch.optim.Optimizer):
         lib = _lib.load()
         ws = torch.empty(lib.e2a_adamw_workspace_bytes(count), dtype=torch.uint8, device=flat.device)
         check(lib.e2a_adamw_step(
-            _address(at), _address(grads), _address(numel), _address(offset), _address(slot), count, code, flat.bits,
-            m, v, ms, vs, flat.elements, step, lr, lr_at, beta1, beta2, group["eps"], group["weight_decay"],
+            at, grads, numel, offset, slot, count, code, flat.bits, m, v, ms, vs, flat.elements, step, lr, lr_at, beta1, beta2, group["eps"], group["weight_decay"],
             None if norm is None else norm.data_ptr(), self.max_grad_norm or 0.0, ws.data_ptr(), ws.numel(),
             stream_of(flat.device)), "e2a_adamw_step")
