@@ -1,5 +1,6 @@
 """What ``ubio_molfm_b200.optim.AdamW`` does with parameters and states that change between its steps."""
 import collections
+import copy
 
 import pytest
 import torch
@@ -142,3 +143,18 @@ def test_a_list_that_grows_or_shrinks():
     before = ps[0].detach().clone()
     opt.step()
     assert torch.equal(ps[0], before) and int(opt.state[ps[1]]["step"]) == 3 and int(opt.state[late]["step"]) == 2
+
+
+@pytest.mark.gpu
+def test_a_saved_state_of_other_shapes_is_refused():
+    from ubio_molfm_b200.optim import AdamW
+
+    ps, opt = _pair([600, 30], 8)
+    opt.step()
+    for key in ("exp_avg_scale", "exp_avg_sq_scale", "step"):
+        held = copy.deepcopy(opt.state_dict())
+        held["state"][0][key] = held["state"][0][key].reshape(-1)[:1] if key != "step" else torch.ones(2)
+        other = AdamW(ps, lr=0.5, state_bits=8)
+        with pytest.raises(ValueError, match="shape"):
+            other.load_state_dict(held)
+        assert other.param_groups[0]["lr"] == 0.5 and not other.state

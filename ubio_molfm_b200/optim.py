@@ -280,11 +280,13 @@ class AdamW(torch.optim.Optimizer):
         for k, s in held.items():
             if set(s) != wanted or s["exp_avg"].dtype != kind or s["exp_avg_sq"].dtype != kind:
                 raise ValueError(f"state of parameter {k} is not one of {self.state_bits}-bit moments")
-        pairs = [(i, k, p) for g, mine in zip(groups, self.param_groups)
-                 for k, (i, p) in enumerate(zip(g["params"], mine["params"]))]
-        for i, _, p in pairs:
-            if i in held and (held[i]["exp_avg"].shape != p.shape or held[i]["exp_avg_sq"].shape != p.shape):
-                raise ValueError(f"state of parameter {i} has another shape than the parameter")
+        pairs = [(i, p) for g, mine in zip(groups, self.param_groups) for i, p in zip(g["params"], mine["params"])]
+        for i, p in pairs:
+            scales = (-(-p.numel() // BLOCK),)
+            shapes = {"step": (), "exp_avg": p.shape, "exp_avg_sq": p.shape, "exp_avg_scale": scales,
+                      "exp_avg_sq_scale": scales}
+            if i in held and any(t.shape != shapes[k] for k, t in held[i].items()):
+                raise ValueError(f"state of parameter {i} has another shape than the parameter's")
         super().load_state_dict({"state": {}, "param_groups": groups})    # checks and takes the groups
         for gi, (g, mine) in enumerate(zip(groups, self.param_groups)):
             if any(i in held for i in g["params"]):
