@@ -158,3 +158,27 @@ def test_a_saved_state_of_other_shapes_is_refused():
         with pytest.raises(ValueError, match="shape"):
             other.load_state_dict(held)
         assert other.param_groups[0]["lr"] == 0.5 and not other.state
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("when", ["new", "cleared"])
+def test_state_is_not_made_inside_a_capture(bits, when):
+    """Its zeros would be captured and every replay would start from them."""
+    ps, opt = _pair([300, 20], bits)
+    if when == "cleared":
+        opt.step()
+        opt.state.clear()
+    before = [p.detach().clone() for p in ps]
+    with pytest.raises(RuntimeError, match="flat_state"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, b) for p, b in zip(ps, before))
+    opt.flat_state()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for t in (1, 2):
+        graph.replay()
+        assert int(opt.state[ps[0]]["step"]) == t

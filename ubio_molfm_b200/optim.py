@@ -241,6 +241,9 @@ class AdamW(torch.optim.Optimizer):
     def _lay_out(self, i):
         """A flat state for group ``i``, with what ``state`` has for its parameters and zeros for the others."""
         params = self.param_groups[i]["params"]
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW's state would be made inside a graph capture, and made anew by every replay: call "
+                               "flat_state() for each group before it")
         flat = _Flat(params, self.state_bits)
         with torch.no_grad():
             for k, p in enumerate(params):
