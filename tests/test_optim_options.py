@@ -52,3 +52,37 @@ def test_the_smallest_epsilon(bits):
     AdamW([q], lr=1e-2, eps=1e-30, weight_decay=0.0, state_bits=bits).step()
     assert torch.equal(p[::3], before[::3])
     assert float((p - q).detach().abs().max()) <= 16 * 2.0 ** -24 * 4       # |p| + |update| <= 4 here
+
+
+@pytest.mark.parametrize("option", [dict(maximize=True), dict(amsgrad=True), dict(differentiable=True),
+                                    dict(decoupled_weight_decay=False), dict(state_bits=8), dict(max_grad_norm=1.0)])
+def test_options_that_it_does_not_have_are_refused(option):
+    from ubio_molfm_b200.optim import AdamW
+
+    p, q = (torch.nn.Parameter(torch.zeros(3)) for _ in range(2))
+    with pytest.raises(ValueError, match=next(iter(option))):
+        AdamW([dict(params=[p], **option)])
+    opt = AdamW([p])
+    with pytest.raises(ValueError, match=next(iter(option))):
+        opt.add_param_group(dict(params=[q], **option))
+    assert len(opt.param_groups) == 1
+    held = opt.state_dict()
+    held["param_groups"][0].update(option)
+    with pytest.raises(ValueError, match=next(iter(option))):
+        opt.load_state_dict(held)
+    opt.param_groups[0].update(option)
+    p.grad = torch.ones(3)
+    with pytest.raises(ValueError, match=next(iter(option))):
+        opt.step()
+
+
+def test_options_that_change_nothing_are_taken():
+    """PyTorch's own AdamW state without them set, a scheduler's keys, a user's own."""
+    from ubio_molfm_b200.optim import AdamW
+
+    p = torch.nn.Parameter(torch.zeros(3))
+    theirs = torch.optim.AdamW([p], lr=0.5)
+    opt = AdamW([dict(params=[p], name="head", initial_lr=1e-3)])
+    opt.load_state_dict(theirs.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.5
+    opt.step()

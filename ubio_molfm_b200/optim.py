@@ -172,6 +172,17 @@ class _Flat:
             mine[k].copy_(t)
 
 
+# group options that change PyTorch's AdamW or this one's arguments, with the only value that they may have here
+_FIXED = {"maximize": False, "amsgrad": False, "differentiable": False, "decoupled_weight_decay": True,
+          "state_bits": None, "max_grad_norm": None}
+
+
+def _check_options(group):
+    for k, only in _FIXED.items():
+        if k in group and (only is None or bool(group[k]) != only):
+            raise ValueError(f"AdamW takes no {k}={group[k]!r} for a group")
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) with PyTorch's arguments and update; parameters in float32, bfloat16 or
     float16, contiguous, the arithmetic in fp32 with one rounding to the parameter's type; ``eps`` is 0 or at least
@@ -186,6 +197,9 @@ class AdamW(torch.optim.Optimizer):
       tensor on the device).  A step whose norm is not finite changes nothing, step counts included.
     * ``lr`` of a group: a float, or a float32 tensor of one element on the parameters' device, which a captured
       step reads anew at every replay.
+
+    A group's options that would change the update and that there are none of here (``maximize``, ``amsgrad``,
+    ``differentiable``, ``decoupled_weight_decay=False``) are refused, in a loaded state too.
 
     Parameters without a gradient are left out of a step, each has its own step count.  State entries
     (``step``, ``exp_avg``, ``exp_avg_sq`` and, in 8 bits, their ``_scale``) are views of one flat buffer per
@@ -207,6 +221,7 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
         g = self.param_groups[-1]
         try:
+            _check_options(g)
             b1, b2 = g["betas"]
             if not (0 <= b1 < 1 and 0 <= b2 < 1 and g["eps"] >= 0 and g["weight_decay"] >= 0):
                 raise ValueError(f"invalid betas {g['betas']}, eps {g['eps']} or weight_decay {g['weight_decay']}")
@@ -277,6 +292,8 @@ class AdamW(torch.optim.Optimizer):
         """Restores types and bits as they were saved; a state of other bits or shapes is refused."""
         groups = state_dict["param_groups"]
         held = state_dict["state"]
+        for g in groups:
+            _check_options(g)
         wanted = {"step", "exp_avg", "exp_avg_sq"} | (
             {"exp_avg_scale", "exp_avg_sq_scale"} if self.state_bits == 8 else set())
         kind = torch.float32 if self.state_bits == 32 else torch.uint8
@@ -339,6 +356,7 @@ class AdamW(torch.optim.Optimizer):
         """The launches of a group: ``[(group, flat state, type code, number of tensors, and where the addresses of the
         parameters and of their gradients, their sizes, state offsets and slots stand)]``; ``keep`` holds what has to
         live until then."""
+        _check_options(group)
         params = group["params"]
         if not params:
             return []
