@@ -86,3 +86,16 @@ def test_options_that_change_nothing_are_taken():
     opt.load_state_dict(theirs.state_dict())
     assert opt.param_groups[0]["lr"] == 0.5
     opt.step()
+
+
+@pytest.mark.gpu
+def test_a_refused_learning_rate_leaves_all_groups_as_they_were():
+    from ubio_molfm_b200.optim import AdamW
+
+    ps = [_param(30, 1), _param(40, 2)]
+    opt = AdamW([dict(params=[ps[0]]), dict(params=[ps[1]], lr=torch.tensor(1e-3, dtype=torch.float64, device=DEV))])
+    before, versions = [p.detach().clone() for p in ps], [p._version for p in ps]
+    with pytest.raises(ValueError, match="lr"):
+        opt.step()
+    assert all(torch.equal(p, b) for p, b in zip(ps, before)) and int(opt.flat_state(0)["step"]) == 0
+    assert ps[1]._version == versions[1]

@@ -120,6 +120,15 @@ def grad_norm(tensors):
         return _norm(dev, [(code, n, _address(at), _address(numel)) for code, n, at, numel in tables])
 
 
+def _rate(lr, device):
+    """``(value, device address or None)`` of a group's learning rate."""
+    if not isinstance(lr, torch.Tensor) or not lr.is_cuda:
+        return float(lr), None
+    if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != device:
+        raise ValueError("a tensor lr must be one float32 value on the parameters' device")
+    return 0.0, lr.data_ptr()
+
+
 class _Flat:
     """The state of one parameter group: flat moments, every tensor at a multiple of 256 elements, and a step
     count per tensor."""
@@ -343,7 +352,7 @@ class AdamW(torch.optim.Optimizer):
             if any(w[1].device != dev for w in work):
                 raise ValueError("the parameters to clip together are on more than one device")
             with torch.cuda.device(dev):
-                norm = self.last_grad_norm = _norm(dev, [(w[2], w[3], w[5], w[6]) for w in work])
+                norm = self.last_grad_norm = _norm(dev, [(w[3], w[4], w[6], w[7]) for w in work])
         for w in work:
             if w[1].device.index == torch.cuda.current_device():
                 self._launch(*w, norm)
@@ -353,9 +362,9 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _group_work(self, gi, group, keep):
-        """The launches of a group: ``[(group, flat state, type code, number of tensors, and where the addresses of the
-        parameters and of their gradients, their sizes, state offsets and slots stand)]``; ``keep`` holds what has to
-        live until then."""
+        """The launches of a group: ``[(group, flat state, learning rate, type code, number of tensors, and where the
+        addresses of the parameters and of their gradients, their sizes, state offsets and slots stand)]``; ``keep``
+        holds what has to live until then."""
         _check_options(group)
         params = group["params"]
         if not params:
@@ -365,10 +374,11 @@ class AdamW(torch.optim.Optimizer):
             if all(p.grad is None for p in params):
                 return []
             flat = self._lay_out(gi)
-        found = self._read(group, flat, keep)
+        rate = _rate(group["lr"], flat.device)
+        found = self._read(group, flat, rate, keep)
         if found is None and not flat.belongs_to(params):
             flat = self._lay_out(gi)
-            found = self._read(group, flat, keep)
+            found = self._read(group, flat, rate, keep)
         if found is not None:
             return found
         index = [k for k, p in enumerate(params) if p.grad is not None]
@@ -387,13 +397,13 @@ class AdamW(torch.optim.Optimizer):
             table = [_pointers(ps), _pointers(gs), *(array(a.typecode, [a[k] for k in ks])
                                                      for a in (flat.numel, flat.offset, flat.slot))]
             keep.append((grads, table))
-            work.append((group, flat, code, len(ps), *map(_address, table)))
+            work.append((group, flat, rate, code, len(ps), *map(_address, table)))
         # the kernels write behind autograd's back: saved tensors and caches keyed on versions have to see it
         torch.autograd.graph.increment_version(params)
         return work
 
     @staticmethod
-    def _read(group, flat, keep):
+    def _read(group, flat, rate, keep):
         """The launch of a group whose parameters are those of ``flat`` and all alike, in one call; else None."""
         params, n = group["params"], len(flat.params)
         table = _zeros("q", 5 * n + 2)
@@ -406,22 +416,16 @@ class AdamW(torch.optim.Optimizer):
         if two[1] != flat.device.index:
             raise ValueError("the parameters have moved to another device than their state")
         keep.append(table)
-        return [(group, flat, two[0], count, at, at + 8 * n, at + 16 * n, at + 24 * n, at + 32 * n)]
+        return [(group, flat, rate, two[0], count, at, at + 8 * n, at + 16 * n, at + 24 * n, at + 32 * n)]
 
-    def _launch(self, group, flat, code, count, at, grads, numel, offset, slot, norm):
-        lr, lr_at = group["lr"], None
-        if isinstance(lr, torch.Tensor) and lr.is_cuda:
-            if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != flat.device:
-                raise ValueError("a tensor lr must be one float32 value on the parameters' device")
-            lr, lr_at = 0.0, lr.data_ptr()
-        else:
-            lr = float(lr)
+    def _launch(self, group, flat, rate, code, count, at, grads, numel, offset, slot, norm):
         (beta1, beta2), b = group["betas"], flat.buffers
         m, v, ms, vs, step = (b[k].data_ptr() if k in b else None for k in (
             "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "step"))
         lib = _lib.load()
         ws = torch.empty(lib.e2a_adamw_workspace_bytes(count), dtype=torch.uint8, device=flat.device)
         check(lib.e2a_adamw_step(
-            at, grads, numel, offset, slot, count, code, flat.bits, m, v, ms, vs, flat.elements, step, lr, lr_at, beta1, beta2, group["eps"], group["weight_decay"],
+            at, grads, numel, offset, slot, count, code, flat.bits, m, v, ms, vs, flat.elements, step, *rate, beta1,
+            beta2, group["eps"], group["weight_decay"],
             None if norm is None else norm.data_ptr(), self.max_grad_norm or 0.0, ws.data_ptr(), ws.numel(),
             stream_of(flat.device)), "e2a_adamw_step")
