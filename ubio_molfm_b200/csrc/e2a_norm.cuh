@@ -16,9 +16,9 @@
 // 100, 161 and 243 us, that is 6.5, 6.1 and 6.7 TB/s where a copy runs at 6.5; 97,865 x 512 fp32: 65 and 93 us;
 // 16,384 x 4,096 bf16 without activation: 49 and 82 us (5.5 and 4.9 TB/s: one row a CTA, its sums behind barriers).
 //
-// The statistics are two-pass in fp32 and kept per row.  Column sums: a thread's own rows in fp32 chains of at most
+// The statistics are two-pass in fp32, of the differences to the row's first value, and kept per row.  Column sums: a thread's own rows in fp32 chains of at most
 // 128, which join the CTA's partial rows in memory; those are added up in CTA order in 64 bits.  No atomics.  Rows
-// of more than 8,192 values take loops over memory (first part below), whose column sums are in 64 bits throughout.
+// of more than 8,192 values take loops over memory (first part below), whose sums are in 64 bits throughout.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -87,6 +87,32 @@ struct Norm {
 
 __device__ __forceinline__ float at(const float* v, int64_t c, float without) { return v ? __ldg(v + c) : without; }
 
+// Means over a row's columns, by a warp: f(c, p) adds column c's terms to p.  AT_ONCE of them (a few at the row's end) add
+// up in fp32, the rest in 64 bits.
+template <int AT_ONCE, int K, typename F>
+__device__ __forceinline__ void row_means(int64_t W, double (&mean)[K], F f) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) mean[k] = 0.;
+  int64_t c = threadIdx.x & 31;
+  for (; c + 32 * (AT_ONCE - 1) < W; c += 32 * AT_ONCE) {
+    float p[K] = {};
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) f(c + 32 * j, p);
+#pragma unroll
+    for (int k = 0; k < K; ++k) mean[k] += p[k];
+  }
+  float p[K] = {};
+  for (; c < W; c += 32) f(c, p);
+#pragma unroll
+  for (int k = 0; k < K; ++k) mean[k] += p[k];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mean[k] += __shfl_xor_sync(0xffffffffu, mean[k], o);
+    mean[k] /= W;
+  }
+}
+
 template <typename T>
 __global__ void k_ln_fwd(const T* __restrict__ x, int64_t ldx, Norm n, int64_t rows, float eps, T* __restrict__ y,
                          float* __restrict__ mean_out, float* __restrict__ rstd_out) {
@@ -94,17 +120,17 @@ __global__ void k_ln_fwd(const T* __restrict__ x, int64_t ldx, Norm n, int64_t r
   const int64_t nw = ((int64_t)gridDim.x * blockDim.x) >> 5;
   for (int64_t r = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5; r < rows; r += nw) {
     const T* xr = x + r * ldx;
-    float s = 0.f;
-    for (int64_t c = lane; c < n.W; c += 32) s += to_f(xr[c]);
-    const float mean = e2a_warp_sum(s) / n.W;
-    float v = 0.f;
+    const float x0 = to_f(xr[0]);      // see k_row_fwd
+    double shift[1], var[1];
+    row_means<8>(n.W, shift, [&](int64_t c, float* p) { p[0] += to_f(xr[c]) - x0; });
+    const float by = (float)shift[0], mean = x0 + by;
+    row_means<8>(n.W, var, [&](int64_t c, float* p) {
+      const float d = (to_f(xr[c]) - x0) - by;
+      p[0] = fmaf(d, d, p[0]);
+    });
+    const float rstd = (float)rsqrt(var[0] + eps);
     for (int64_t c = lane; c < n.W; c += 32) {
-      const float d = to_f(xr[c]) - mean;
-      v += d * d;
-    }
-    const float rstd = rsqrtf(e2a_warp_sum(v) / n.W + eps);
-    for (int64_t c = lane; c < n.W; c += 32) {
-      const float z = (to_f(xr[c]) - mean) * rstd * at(n.gamma, c, 1.f) + at(n.beta, c, 0.f);
+      const float z = ((to_f(xr[c]) - x0) - by) * rstd * at(n.gamma, c, 1.f) + at(n.beta, c, 0.f);
       y[r * n.W + c] = from_f<T>(activation(z, n.silu).y);
     }
     if (lane == 0) {
@@ -124,15 +150,14 @@ __global__ void k_ln_bwd(const T* __restrict__ x, int64_t ldx, const T* __restri
     const T* xr = x + r * ldx;
     const T* gr = g + r * ldg;
     const float mean = mean_in[r], rstd = rstd_in[r];
-    float s1 = 0.f, s2 = 0.f;
-    for (int64_t c = lane; c < n.W; c += 32) {
+    double m[2];
+    row_means<4>(n.W, m, [&](int64_t c, float* p) {
       const float w = at(n.gamma, c, 1.f), xh = (to_f(xr[c]) - mean) * rstd;
       const float h = to_f(gr[c]) * activation(xh * w + at(n.beta, c, 0.f), n.silu).d1 * w;
-      s1 += h;
-      s2 += h * xh;
-    }
-    s1 = e2a_warp_sum(s1) / n.W;
-    s2 = e2a_warp_sum(s2) / n.W;
+      p[0] += h;
+      p[1] = fmaf(h, xh, p[1]);
+    });
+    const float s1 = (float)m[0], s2 = (float)m[1];
     for (int64_t c = lane; c < n.W; c += 32) {
       const float w = at(n.gamma, c, 1.f), xh = (to_f(xr[c]) - mean) * rstd;
       const float h = to_f(gr[c]) * activation(xh * w + at(n.beta, c, 0.f), n.silu).d1 * w;
@@ -153,42 +178,41 @@ __global__ void k_ln_bwd2(const T* __restrict__ x, int64_t ldx, const T* __restr
     const T* gr = g + r * ldg;
     const T* ur = u + r * ldu;
     const float mean = mean_in[r], rstd = rstd_in[r];
-    float su = 0.f, sc = 0.f, s1 = 0.f, s2 = 0.f, su2 = 0.f;
-    for (int64_t c = lane; c < n.W; c += 32) {
+    double m[5], e[2];
+    row_means<4>(n.W, m, [&](int64_t c, float* p) {
       const float w = at(n.gamma, c, 1.f), xh = (to_f(xr[c]) - mean) * rstd, uv = to_f(ur[c]);
       const float h = to_f(gr[c]) * activation(xh * w + at(n.beta, c, 0.f), n.silu).d1 * w;
-      su += uv;
-      sc += uv * xh;
-      s1 += h;
-      s2 += h * xh;
-      su2 += h * uv;
-    }
-    su = e2a_warp_sum(su) / n.W;
-    sc = e2a_warp_sum(sc) / n.W;
-    s1 = e2a_warp_sum(s1) / n.W;
-    s2 = e2a_warp_sum(s2) / n.W;
-    const float ht = rstd * (e2a_warp_sum(su2) / n.W - s1 * su - s2 * sc);
-    float k1 = 0.f, k2 = 0.f;
-    for (int pass = 0; pass < 2; ++pass) {
-      if (pass == 1) {
-        k1 = e2a_warp_sum(k1) / n.W;
-        k2 = e2a_warp_sum(k2) / n.W + ht;
-      }
-      for (int64_t c = lane; c < n.W; c += 32) {
-        const float w = at(n.gamma, c, 1.f), xh = (to_f(xr[c]) - mean) * rstd, uv = to_f(ur[c]), gv = to_f(gr[c]);
-        const Act a = activation(xh * w + at(n.beta, c, 0.f), n.silu);
-        const float pc = at(n.p, c, 0.f), t = rstd * (uv - su - xh * sc);
-        const float v = w * t + pc * xh + at(n.q, c, 0.f);
-        const float ga = gv * a.d1;
-        const float k = gv * a.d2 * v * w + ga * pc - rstd * (uv * s2 + ga * w * sc);
-        if (pass == 0) {
-          k1 += k;
-          k2 += k * xh;
-        } else {
-          dg[r * n.W + c] = from_f<T>(a.d1 * v);
-          dx[r * n.W + c] = from_f<T>(rstd * (k - k1 - xh * k2));
-        }
-      }
+      p[0] += uv;
+      p[1] = fmaf(uv, xh, p[1]);
+      p[2] += h;
+      p[3] = fmaf(h, xh, p[3]);
+      p[4] = fmaf(h, uv, p[4]);
+    });
+    const float su = (float)m[0], sc = (float)m[1], s2 = (float)m[3];
+    const double ht = rstd * (m[4] - m[2] * m[0] - m[3] * m[1]);
+    // one column's dg and k
+    const auto column = [&](int64_t c, float* xh, float* dgv) {
+      *xh = (to_f(xr[c]) - mean) * rstd;
+      const float w = at(n.gamma, c, 1.f), uv = to_f(ur[c]), gv = to_f(gr[c]);
+      const Act a = activation(*xh * w + at(n.beta, c, 0.f), n.silu);
+      const float pc = at(n.p, c, 0.f), t = rstd * (uv - su - *xh * sc);
+      const float v = w * t + pc * *xh + at(n.q, c, 0.f);
+      const float ga = gv * a.d1;
+      *dgv = a.d1 * v;
+      return gv * a.d2 * v * w + ga * pc - rstd * (uv * s2 + ga * w * sc);
+    };
+    row_means<2>(n.W, e, [&](int64_t c, float* p) {
+      float xh, dgv;
+      const float k = column(c, &xh, &dgv);
+      p[0] += k;
+      p[1] = fmaf(k, xh, p[1]);
+    });
+    const float k1 = (float)e[0], k2 = (float)(e[1] + ht);
+    for (int64_t c = lane; c < n.W; c += 32) {
+      float xh, dgv;
+      const float k = column(c, &xh, &dgv);
+      dg[r * n.W + c] = from_f<T>(dgv);
+      dx[r * n.W + c] = from_f<T>(rstd * (k - k1 - xh * k2));
     }
     if (lane == 0) {
       row_u[r] = su;
@@ -392,6 +416,18 @@ __device__ __forceinline__ void columns(const float* p, int W, float without, fl
   }
 }
 
+// Sets a thread's values beyond the row's end.
+template <class S>
+__device__ __forceinline__ void fill_beyond(float (&v)[S::N], int W, float value) {
+#pragma unroll
+  for (int i = 0; i < S::V; ++i) {
+    if (((int)(threadIdx.x % S::TEAM) + S::TEAM * i) * S::VEC >= W) {
+#pragma unroll
+      for (int k = 0; k < S::VEC; ++k) v[i * S::VEC + k] = value;
+    }
+  }
+}
+
 template <class S, bool SILU>
 __global__ void __launch_bounds__(S::THREADS)
 k_row_fwd(const typename S::T* __restrict__ x, int64_t ldx, Norm n, int64_t rows, float eps,
@@ -405,28 +441,35 @@ k_row_fwd(const typename S::T* __restrict__ x, int64_t ldx, Norm n, int64_t rows
   int64_t row = blockIdx.x * (int64_t)S::TEAMS + threadIdx.x / S::TEAM;
   Rows<S, 1> in{{x}, {ldx}, rows, step, W};
   in.load(row);
+  // The statistics are those of the differences to the row's first value, which are exact for values near each other:
+  // no error grows with the mean, and a row of one value, whatever it is, has variance 0.
+  typename S::T first{};
+  if (S::TEAM > 32 && row < rows) first = __ldg(x + row * ldx);
   for (int64_t base = blockIdx.x * (int64_t)S::TEAMS; base < rows; base += step, row += step) {
     alignas(8) float v[1][S::N];
     in.take(row, v);
+    float x0;
+    if (S::TEAM > 32) {
+      x0 = to_f(first);
+      if (row + step < rows) first = __ldg(x + (row + step) * ldx);
+    } else {
+      x0 = __shfl_sync(0xffffffffu, v[0][0], 0, S::TEAM < 32 ? S::TEAM : 32);
+    }
+    fill_beyond<S>(v[0], W, x0);
     float2 two = f2(0.f);
 #pragma unroll
-    for (int e = 0; e < S::N / 2; ++e) two = f2_add(two, E2A_PAIR(v[0], e));
+    for (int e = 0; e < S::N / 2; ++e) {
+      E2A_PAIR(v[0], e) = f2_add(E2A_PAIR(v[0], e), f2(-x0));
+      two = f2_add(two, E2A_PAIR(v[0], e));
+    }
     float sum[1] = {two.x + two.y};
     team_sum<S::TEAM>(sum, sh, turn);
-    // corrected by what the product with 1 / W leaves: a row of one value has that mean where its sum is exact
-    // (a division there cost the 16,384 x 4,096 bf16 rows a fifth)
-    const float rough = sum[0] * inv, mean = fmaf(fmaf(-rough, (float)W, sum[0]), inv, rough);
+    const float shift = sum[0] * inv, mean = x0 + shift;
+    fill_beyond<S>(v[0], W, shift);
     two = f2(0.f);
 #pragma unroll
-    for (int i = 0; i < S::V; ++i) {
-      if ((me + S::TEAM * i) * S::VEC >= W) {       // beyond the row's end: as if it were the mean
-#pragma unroll
-        for (int k = 0; k < S::VEC; ++k) v[0][i * S::VEC + k] = mean;
-      }
-    }
-#pragma unroll
     for (int e = 0; e < S::N / 2; ++e) {
-      E2A_PAIR(v[0], e) = f2_add(E2A_PAIR(v[0], e), f2(-mean));
+      E2A_PAIR(v[0], e) = f2_add(E2A_PAIR(v[0], e), f2(-shift));
       two = f2_fma(E2A_PAIR(v[0], e), E2A_PAIR(v[0], e), two);
     }
     sum[0] = two.x + two.y;
