@@ -99,3 +99,20 @@ def test_gradients_of_constant_and_nearly_constant_rows(width, dtype):
     major = _majorants_with(_per(x, constant), x, w, b, g, u, p, q)
     for k, t in _run(x, w, b, True, g, (u, p, q)).items():
         _close(t, ref[k], major[k], k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [1, 3, 12, 100, 128, 1000, 6001, 9001])
+@pytest.mark.parametrize("value", [2e36, 1e38, -3.4028234663852886e38])
+def test_rows_of_one_extreme_value(width, value):
+    """The type's lowest value as a mask leaves it, and others whose sum or product with 1 / sqrt(eps) passes fp32's
+    range: xh is 0, y the activated bias, and the gradients are those of xh = 0."""
+    _, w, b, g, u, p, q = _inputs(4, width, torch.float32)
+    x = torch.full((4, width), value, device=DEV)
+    ref = reference(torch.zeros_like(x), w, b, True, g, u, p, q)
+    zero = torch.zeros_like(x)
+    major = _majorants_with(_per(zero, zero[:, :1] == 0), zero, w, b, g, u, p, q)
+    for k, t in _run(x, w, b, True, g, (u, p, q)).items():
+        _close(t, ref[k], major[k], k)
+    y = _run(x, w, b, False, g)["y"]
+    assert torch.equal(y, b.expand(4, width))

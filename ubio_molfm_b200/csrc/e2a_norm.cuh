@@ -368,6 +368,12 @@ struct Shape {
   static constexpr int THREADS = TEAM > 32 ? TEAM : 256;
   static constexpr int TEAMS = THREADS / TEAM;   // rows that a CTA holds at a time
   static constexpr int N = VEC * V;
+  // vectors of a thread that are never beyond the row's end: by_shape takes every shape but the narrowest (a single
+  // vector, or four single values in a team of 8) for rows that fill more than half of it
+  static constexpr int SURE = VEC == 1 && TEAM == 8 ? 0 : V / 2;
+  // those of them that are loaded and stored without asking (150,000 x 262 fp32 second order 275 -> 243 us; with 16-byte
+  // vectors the registers fall worse: 16,384 x 4,096 bf16 157 -> 230 us)
+  static constexpr int UNASKED = VEC == 1 ? SURE : 0;
   static constexpr int SCRATCH = TEAM > 32 ? 2 * 5 * (TEAM / 32) : 1;                    // team_sum
 };
 
@@ -388,7 +394,7 @@ struct Rows {
 #pragma unroll
       for (int i = 0; i < S::V; ++i) {
         const int c = (threadIdx.x % S::TEAM + S::TEAM * i) * S::VEC;
-        next[k][i] = row < rows && c < W ? __ldg(reinterpret_cast<const Raw*>(p[k] + row * ld[k] + c)) : Raw{};
+        next[k][i] = row < rows && (i < S::UNASKED || c < W) ? __ldg(reinterpret_cast<const Raw*>(p[k] + row * ld[k] + c)) : Raw{};
       }
     }
   }
@@ -412,7 +418,7 @@ __device__ __forceinline__ void columns(const float* p, int W, float without, fl
 #pragma unroll
   for (int i = 0; i < S::V; ++i) {
     const int c = (threadIdx.x % S::TEAM + S::TEAM * i) * S::VEC;
-    load_affine<S::VEC>(c < W ? p : nullptr, c, without, v + i * S::VEC);
+    load_affine<S::VEC>(i < S::UNASKED || c < W ? p : nullptr, c, without, v + i * S::VEC);
   }
 }
 
@@ -420,7 +426,7 @@ __device__ __forceinline__ void columns(const float* p, int W, float without, fl
 template <class S>
 __device__ __forceinline__ void fill_beyond(float (&v)[S::N], int W, float value) {
 #pragma unroll
-  for (int i = 0; i < S::V; ++i) {
+  for (int i = S::SURE; i < S::V; ++i) {
     if (((int)(threadIdx.x % S::TEAM) + S::TEAM * i) * S::VEC >= W) {
 #pragma unroll
       for (int k = 0; k < S::VEC; ++k) v[i * S::VEC + k] = value;
@@ -498,7 +504,7 @@ k_row_fwd(const typename S::T* __restrict__ x, int64_t ldx, Norm n, int64_t rows
 #pragma unroll
     for (int i = 0; i < S::V; ++i) {
       const int c = (me + S::TEAM * i) * S::VEC;
-      if (c < W) *reinterpret_cast<Raw*>(y + row * W + c) = S::P::narrow(v[0] + i * S::VEC);
+      if (i < S::UNASKED || c < W) *reinterpret_cast<Raw*>(y + row * W + c) = S::P::narrow(v[0] + i * S::VEC);
     }
   }
 }
@@ -561,7 +567,28 @@ struct Stats {
   }
 };
 
-// part NULL: dx alone; dx NULL: the column sums alone.  Beyond a row's end x is taken for the mean and g for 0.
+// Pair e of a row's normalised values, from x: 0 beyond the row's end, where x counts as 0 and mean rstd can pass fp32's
+// range (a row of one huge value).  There the mean is taken for 0 (MEAN) or the result; which of them costs registers
+// differs: 640,210 x 128 fp32 second order 256 against 265 us, 16,384 x 4,096 bf16 backward 105 against 92 us.
+template <class S, bool MEAN>
+__device__ __forceinline__ float2 normalised(float2 x, int e, int W, const Stats& st) {
+  float2 less = f2(-st.mean);
+  bool beyond[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int i = (2 * e + k) / S::VEC;
+    beyond[k] = i >= S::SURE && ((int)(threadIdx.x % S::TEAM) + S::TEAM * i) * S::VEC >= W;
+    if (MEAN && beyond[k]) (k ? less.y : less.x) = 0.f;
+  }
+  float2 xh = f2_mul(f2_add(x, less), f2(st.rstd));
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (!MEAN && beyond[k]) (k ? xh.y : xh.x) = 0.f;
+  }
+  return xh;
+}
+
+// part NULL: dx alone; dx NULL: the column sums alone.  Beyond a row's end g is 0: so are a and h.
 template <class S, bool SILU>
 __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS)
 k_row_bwd(const typename S::T* __restrict__ x, int64_t ldx, const typename S::T* __restrict__ g, int64_t ldg, Norm n,
@@ -589,7 +616,7 @@ k_row_bwd(const typename S::T* __restrict__ x, int64_t ldx, const typename S::T*
     operands.take(row, v);
     const Stats st = next;
     next.load(mean_in, rstd_in, row + step, rows);
-    columns<S>(n.gamma, W, 0.f, ga);      // beyond the row's end g is 0: so are its a and h
+    columns<S>(n.gamma, W, 0.f, ga);
     if (SILU) columns<S>(n.beta, W, 0.f, be);
     if (!n.gamma) {
 #pragma unroll
@@ -599,7 +626,7 @@ k_row_bwd(const typename S::T* __restrict__ x, int64_t ldx, const typename S::T*
 #pragma unroll
     for (int e = 0; e < S::N / 2; ++e) {
       float2 &xh = E2A_PAIR(v[0], e), &h = E2A_PAIR(v[1], e);
-      xh = f2_mul(f2_add(xh, f2(-st.mean)), f2(st.rstd));
+      xh = normalised<S, false>(xh, e, W, st);
       if (SILU) h = f2_mul(h, derivatives<SILU, false>(f2_fma(xh, E2A_PAIR(ga, e), E2A_PAIR(be, e))).d1);
       E2A_PAIR(dw, e) = f2_fma(h, xh, E2A_PAIR(dw, e));
       E2A_PAIR(db, e) = f2_add(h, E2A_PAIR(db, e));
@@ -617,7 +644,7 @@ k_row_bwd(const typename S::T* __restrict__ x, int64_t ldx, const typename S::T*
 #pragma unroll
       for (int i = 0; i < S::V; ++i) {
         const int c = (me + S::TEAM * i) * S::VEC;
-        if (row < rows && c < W) *reinterpret_cast<Raw*>(dx + row * W + c) = S::P::narrow(v[1] + i * S::VEC);
+        if (row < rows && (i < S::UNASKED || c < W)) *reinterpret_cast<Raw*>(dx + row * W + c) = S::P::narrow(v[1] + i * S::VEC);
       }
     }
     if (part && ++held == kChain) {
@@ -669,7 +696,7 @@ k_row_bwd2(const typename S::T* __restrict__ x, int64_t ldx, const typename S::T
     for (int e = 0; e < S::N / 2; ++e) {
       float2& xh = E2A_PAIR(v[0], e);
       const float2 gv = E2A_PAIR(v[1], e), uv = E2A_PAIR(v[2], e), w = E2A_PAIR(ga, e);
-      xh = f2_mul(f2_add(xh, f2(-st.mean)), r);
+      xh = normalised<S, true>(xh, e, W, st);
       const Act2 a = derivatives<SILU, true>(SILU ? f2_fma(xh, w, E2A_PAIR(be, e)) : xh);
       E2A_PAIR(B, e) = SILU ? f2_mul(a.d1, r) : r;
       E2A_PAIR(C, e) = SILU ? f2_mul(f2_mul(gv, a.d2), f2_mul(w, r)) : f2(0.f);
@@ -726,7 +753,7 @@ k_row_bwd2(const typename S::T* __restrict__ x, int64_t ldx, const typename S::T
 #pragma unroll
     for (int i = 0; i < S::V; ++i) {
       const int c = (me + S::TEAM * i) * S::VEC;
-      if (c < W) {
+      if (i < S::UNASKED || c < W) {
         if (in) *reinterpret_cast<Raw*>(dg + row * W + c) = S::P::narrow(v[1] + i * S::VEC);
       } else {
 #pragma unroll
@@ -748,7 +775,7 @@ k_row_bwd2(const typename S::T* __restrict__ x, int64_t ldx, const typename S::T
 #pragma unroll
     for (int i = 0; i < S::V; ++i) {
       const int c = (me + S::TEAM * i) * S::VEC;
-      if (in && c < W) *reinterpret_cast<Raw*>(dx + row * W + c) = S::P::narrow(v[2] + i * S::VEC);
+      if (in && (i < S::UNASKED || c < W)) *reinterpret_cast<Raw*>(dx + row * W + c) = S::P::narrow(v[2] + i * S::VEC);
     }
     if (part && ++held == kChain) {
       flush_cols<S>(dw, db, part, W, first, sh);
