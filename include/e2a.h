@@ -378,6 +378,8 @@ int e2a_node_map_bwd(const float* pos, const float* dA, int64_t n_nodes, const d
 /* d_dy and dx are the gradients of <dx,u> + <dgamma,p> + <dbeta,q> in dy and x, dgamma / dbeta (may */
 /* be NULL) those in gamma and beta.  Column sums in row order, no atomics.                          */
 /* ------------------------------------------------------------------------------------------ */
+/* Row tensors start at multiples of their type's size, vectors at multiples of 4 bytes, workspaces at   */
+/* multiples of 16; anything else is E2A_ERR_ARG.                                                       */
 int e2a_layer_norm_fwd(const void* x, int64_t ldx, int dtype, const float* gamma, const float* beta, int64_t rows,
                        int64_t W, float eps, int act, void* y, float* mean, float* rstd, void* stream);
 size_t e2a_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t W);
@@ -414,6 +416,9 @@ int e2a_layer_norm_bwd2(const void* x, int64_t ldx, const void* dy, int64_t lddy
 /* m and v of n elements (whole blocks) as fp32.  Parameters that share memory with another parameter or  */
 /* a gradient are refused (E2A_ERR_ARG).                                                              */
 /* ------------------------------------------------------------------------------------------ */
+/* Tensors start at multiples of their type's size, fp32 moments, e2a_moments_unpack's outputs and        */
+/* e2a_adamw_step's workspace at multiples of 16 bytes, the norm's workspace of 8, 8-bit moments, counts   */
+/* and scalars of 4; anything else is E2A_ERR_ARG.                                                      */
 size_t e2a_grad_norm_workspace_bytes(int64_t n_tensors);
 int e2a_sum_squares(const uint64_t* tensors, const int64_t* numel, int64_t n_tensors, int dtype, void* workspace,
                     size_t workspace_bytes, int64_t* n_partials, void* stream);

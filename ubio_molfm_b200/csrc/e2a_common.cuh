@@ -22,6 +22,10 @@ void e2a_note_launch();  // counts kernel launches for e2a_launch_count
 
 static inline size_t e2a_align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
+// Whether one of the addresses is no multiple of `a` (a power of two); NULL is one.
+template <typename... P>
+static inline bool e2a_misaligned(size_t a, const P*... p) { return (((uintptr_t)p | ...) & (a - 1)) != 0; }
+
 // Bump allocator over a caller-provided workspace.  Every sub-buffer is 256-byte aligned.
 struct E2aArena {
   char* base;

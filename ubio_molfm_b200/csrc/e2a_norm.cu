@@ -8,6 +8,7 @@ int e2a_layer_norm_fwd(const void* x, int64_t ldx, int dtype, const float* gamma
   if (bad_shape(rows, W, ldx) || bad_mode(dtype, act)) return E2A_ERR_ARG;
   if (rows == 0) return E2A_OK;
   if (!x || !y || !mean || !rstd) return E2A_ERR_ARG;
+  if (bad_rows(dtype, x, y) || e2a_misaligned(4, gamma, beta, mean, rstd)) return E2A_ERR_ARG;
   const Norm n{gamma, beta, nullptr, nullptr, W, act == 1};
   return by_type(dtype, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
@@ -44,6 +45,9 @@ int e2a_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy,
   cudaStream_t st = (cudaStream_t)stream;
   if (rows == 0) return zero_cols(dgamma, dbeta, W, st);
   if (!x || !dy || !mean || !rstd) return E2A_ERR_ARG;
+  if (bad_rows(dtype, x, dy, dx) || e2a_misaligned(4, gamma, beta, mean, rstd, dgamma, dbeta) ||
+      e2a_misaligned(16, workspace))
+    return E2A_ERR_ARG;
   if ((dgamma || dbeta) && (!workspace || workspace_bytes < part_bytes(rows, W))) return E2A_ERR_WORKSPACE;
   const Norm n{gamma, beta, nullptr, nullptr, W, act == 1};
   return by_type(dtype, [&](auto* t) -> int {

@@ -920,6 +920,10 @@ int launch_cols(bool second, const T* x, int64_t ldx, const T* g, int64_t ldg, c
 
 bool bad_shape(int64_t rows, int64_t W, int64_t ld) { return rows < 0 || W <= 0 || W > (1ll << 30) || ld < 0; }
 
+// Rows start at multiples of their type's size, the fp32 vectors and the workspace at multiples of theirs.
+template <typename... P>
+bool bad_rows(int dtype, const P*... p) { return e2a_misaligned(dtype == 0 ? 4 : 2, p...); }
+
 bool bad_mode(int dtype, int act) { return dtype < 0 || dtype > 2 || (act != 0 && act != 1); }
 
 size_t part_bytes(int64_t rows, int64_t W) {

@@ -16,6 +16,9 @@ int e2a_layer_norm_bwd2(const void* x, int64_t ldx, const void* dy, int64_t lddy
   cudaStream_t st = (cudaStream_t)stream;
   if (rows == 0) return zero_cols(dgamma, dbeta, W, st);
   if (!x || !dy || !u || !mean || !rstd || !d_dy || !dx) return E2A_ERR_ARG;
+  if (bad_rows(dtype, x, dy, u, d_dy, dx) || e2a_misaligned(4, gamma, beta, mean, rstd, p, q, dgamma, dbeta) ||
+      e2a_misaligned(16, workspace))
+    return E2A_ERR_ARG;
   E2aArena ar{(char*)workspace, workspace_bytes, 0};
   double* part = (double*)ar.take(part_bytes(rows, W));
   const bool loops = W > kMaxTeamWidth;      // <u> and c of every row, for the column sums' own pass

@@ -653,7 +653,7 @@ size_t e2a_grad_norm_workspace_bytes(int64_t n_tensors) {
 
 int e2a_sum_squares(const uint64_t* tensors, const int64_t* numel, int64_t n_tensors, int dtype, void* workspace,
                     size_t workspace_bytes, int64_t* n_partials, void* stream) {
-  if (bad_tensors(tensors, numel, n_tensors, dtype) || !n_partials) return E2A_ERR_ARG;
+  if (bad_tensors(tensors, numel, n_tensors, dtype) || !n_partials || e2a_misaligned(8, workspace)) return E2A_ERR_ARG;
   *n_partials = 0;
   double* part = (double*)workspace;
   const int64_t room = (int64_t)(workspace_bytes / sizeof(double));
@@ -678,6 +678,7 @@ int e2a_sum_squares(const uint64_t* tensors, const int64_t* numel, int64_t n_ten
 
 int e2a_norm_of_squares(const void* partials, int64_t n_partials, float* norm, void* stream) {
   if (n_partials < 0 || (n_partials > 0 && !partials) || !norm) return E2A_ERR_ARG;
+  if (e2a_misaligned(8, partials) || e2a_misaligned(4, norm)) return E2A_ERR_ARG;
   k_norm<<<1, kThreads, 0, (cudaStream_t)stream>>>((const double*)partials, n_partials, norm);
   E2A_CHECK_LAUNCH();
   return E2A_OK;
@@ -707,6 +708,9 @@ int e2a_adamw_step(const uint64_t* params, const uint64_t* grads, const int64_t*
   if (n_tensors == 0) return E2A_OK;
   if (!state_offset || !slots || !exp_avg || !exp_avg_sq || !step || n_tensors > (1 << 24)) return E2A_ERR_ARG;
   if (state_bits == 8 && (!exp_avg_scale || !exp_avg_sq_scale)) return E2A_ERR_ARG;
+  if (e2a_misaligned(state_bits == 32 ? 16 : 4, exp_avg, exp_avg_sq) ||
+      e2a_misaligned(4, step, lr_device, grad_norm) || e2a_misaligned(16, workspace))
+    return E2A_ERR_ARG;
   int64_t end = 0;
   for (int64_t j = 0; j < n_tensors; ++j) {
     if (state_offset[j] < end || state_offset[j] % kBlock || (j > 0 && slots[j] <= slots[j - 1]) || slots[j] < 0)
@@ -754,7 +758,7 @@ int e2a_moments_unpack(const uint8_t* exp_avg, const uint8_t* exp_avg_sq, const 
   if (n < 0) return E2A_ERR_ARG;
   if (n == 0) return E2A_OK;
   if (!exp_avg || !exp_avg_sq || !exp_avg_scale || !exp_avg_sq_scale || !out_avg || !out_avg_sq) return E2A_ERR_ARG;
-  if (n % kBlock) return E2A_ERR_ARG;
+  if (n % kBlock || e2a_misaligned(4, exp_avg, exp_avg_sq) || e2a_misaligned(16, out_avg, out_avg_sq)) return E2A_ERR_ARG;
   const int64_t b = (n / kBlock + kThreads / 32 - 1) / (kThreads / 32);
   k_moments_unpack<<<(int)(b < 148 * 64 ? b : 148 * 64), kThreads, 0, (cudaStream_t)stream>>>(
       exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, n, out_avg, out_avg_sq);
