@@ -835,12 +835,20 @@ int by_shape(int64_t W, bool vec, F f) {
     if (W <= 16 * VEC) return f(Shape<T, VEC, 2, 8>{});
     if (W <= 32 * VEC) return f(Shape<T, VEC, 2, 16>{});
     if (W <= 64 * VEC) return f(Shape<T, VEC, 2, 32>{});
-    if (W <= 512) return f(Shape<T, VEC, V16, 32>{});
-    if (W <= 32 * WIDE) return f(Shape<T, VEC, VW, 32>{});
+    if constexpr (VEC < 8) {      // 16 values a thread are two vectors otherwise
+      if (W <= 512) return f(Shape<T, VEC, V16, 32>{});
+    }
+    if constexpr (WIDE > 16) {
+      if (W <= 32 * WIDE) return f(Shape<T, VEC, VW, 32>{});
+    }
     if (W <= 64 * WIDE) return f(Shape<T, VEC, VW, 64>{});
     if (W <= 128 * WIDE) return f(Shape<T, VEC, VW, 128>{});
-    if (W <= 256 * WIDE) return f(Shape<T, VEC, VW, 256>{});
-    return f(Shape<T, VEC, V16, 512>{});
+    if constexpr (WIDE > 16) {
+      return f(Shape<T, VEC, VW, 256>{});
+    } else {
+      if (W <= 256 * WIDE) return f(Shape<T, VEC, VW, 256>{});
+      return f(Shape<T, VEC, V16, 512>{});
+    }
   }
   if (W <= 32) return f(Shape<T, 1, 4, 8>{});
   if (W <= 64) return f(Shape<T, 1, 4, 16>{});
@@ -853,12 +861,12 @@ int by_shape(int64_t W, bool vec, F f) {
     if (W <= 1024) return f(Shape<T, 1, 16, 64>{});
     if (W <= 2048) return f(Shape<T, 1, 16, 128>{});
     if (W <= 4096) return f(Shape<T, 1, 16, 256>{});
-    return f(Shape<T, 1, 16, 512>{});
+  } else {
+    if (W <= 512) return f(Shape<T, 1, 8, 64>{});
+    if (W <= 1024) return f(Shape<T, 1, 8, 128>{});
+    if (W <= 2048) return f(Shape<T, 1, 8, 256>{});
+    if (W <= 4096) return f(Shape<T, 1, 8, 512>{});
   }
-  if (W <= 512) return f(Shape<T, 1, 8, 64>{});
-  if (W <= 1024) return f(Shape<T, 1, 8, 128>{});
-  if (W <= 2048) return f(Shape<T, 1, 8, 256>{});
-  if (W <= 4096) return f(Shape<T, 1, 8, 512>{});
   return f(Shape<T, 1, 16, 512>{});
 }
 
