@@ -1,5 +1,59 @@
-// Layer norm: second-order backward entry points (the mathematics and the kernels: e2a_norm.cuh).
+// Layer norm: second-order backward entry points (the mathematics and the kernels: e2a_norm.cuh).  With E2A_ROW_TYPE
+// the kernels for that type of rows, without it the entry points: the compiler works on four parts at once.
 #include "e2a_norm.cuh"
+
+struct E2aLnBwd2 {
+  const void* x; int64_t ldx;
+  const void* dy; int64_t lddy;
+  const void* u; int64_t ldu;
+  const float *gamma, *beta, *mean, *rstd, *p, *q;
+  int64_t rows, W;
+  int act;
+  void *d_dy, *dx;
+  float *dgamma, *dbeta;
+  double* part;
+  float *row_u, *row_c;
+  cudaStream_t st;
+};
+
+template <typename T>
+int e2a_ln_bwd2(const E2aLnBwd2& a);
+
+#ifdef E2A_ROW_TYPE
+
+template <typename T>
+int e2a_ln_bwd2(const E2aLnBwd2& a) {
+  const Norm n{a.gamma, a.beta, a.p, a.q, a.W, a.act == 1};
+  const T *x = (const T*)a.x, *dy = (const T*)a.dy, *u = (const T*)a.u;
+  if (a.W <= kMaxTeamWidth) {
+    const void* of[] = {x, dy, u, a.d_dy, a.dx};
+    const int64_t ld[] = {a.ldx, a.lddy, a.ldu, a.W, a.W};
+    return by_shape<T, 16>(a.W, vectors_fit<T>(n, of, ld, 5), [&](auto shape) -> int {
+      using S = decltype(shape);
+      float* sums = a.dgamma || a.dbeta ? (float*)a.part : nullptr;
+      return by_flag(n.silu, [&](auto silu) -> int {
+        return by_flag(a.p || a.q, [&](auto pq) -> int {
+          constexpr auto kernel = &k_row_bwd2<S, silu.value, pq.value>;
+          int grid = 0;
+          if (const int rc = row_grid<kernel, S>(a.rows, a.W, &grid)) return rc;
+          kernel<<<grid, S::THREADS, 0, a.st>>>(x, a.ldx, dy, a.lddy, u, a.ldu, n, a.mean, a.rstd, a.rows, (T*)a.d_dy,
+                                                (T*)a.dx, sums);
+          E2A_CHECK_LAUNCH();
+          return sums ? sum_parts(sums, grid, a.W, a.dgamma, a.dbeta, a.st) : E2A_OK;
+        });
+      });
+    });
+  }
+  k_ln_bwd2<T><<<grid_rows(a.rows), kThreads, 0, a.st>>>(x, a.ldx, dy, a.lddy, u, a.ldu, n, a.mean, a.rstd, a.rows,
+                                                         (T*)a.d_dy, (T*)a.dx, a.row_u, a.row_c);
+  E2A_CHECK_LAUNCH();
+  if (!a.dgamma && !a.dbeta) return E2A_OK;
+  return launch_cols<T>(true, x, a.ldx, dy, a.lddy, u, a.ldu, n, a.mean, a.rstd, a.row_u, a.row_c, a.rows, a.part,
+                        a.dgamma, a.dbeta, a.st);
+}
+template int e2a_ln_bwd2<E2A_ROW_TYPE>(const E2aLnBwd2&);
+
+#else
 
 extern "C" {
 
@@ -25,35 +79,10 @@ int e2a_layer_norm_bwd2(const void* x, int64_t ldx, const void* dy, int64_t lddy
   float* row_u = loops ? (float*)ar.take(rows * sizeof(float)) : nullptr;
   float* row_c = loops ? (float*)ar.take(rows * sizeof(float)) : nullptr;
   if (!part || (loops && (!row_u || !row_c))) return E2A_ERR_WORKSPACE;
-  const Norm n{gamma, beta, p, q, W, act == 1};
-  return by_type(dtype, [&](auto* t) -> int {
-    using T = std::remove_pointer_t<decltype(t)>;
-    if (W <= kMaxTeamWidth) {
-      const void* of[] = {x, dy, u, d_dy, dx};
-      const int64_t ld[] = {ldx, lddy, ldu, W, W};
-      return by_shape<T, 16>(W, vectors_fit<T>(n, of, ld, 5), [&](auto shape) -> int {
-        using S = decltype(shape);
-        float* sums = dgamma || dbeta ? (float*)part : nullptr;
-        return by_flag(n.silu, [&](auto silu) -> int {
-          return by_flag(p || q, [&](auto pq) -> int {
-            constexpr auto kernel = &k_row_bwd2<S, silu.value, pq.value>;
-            int grid = 0;
-            if (const int rc = row_grid<kernel, S>(rows, W, &grid)) return rc;
-            kernel<<<grid, S::THREADS, 0, st>>>((const T*)x, ldx, (const T*)dy, lddy, (const T*)u, ldu, n, mean, rstd,
-                                                    rows, (T*)d_dy, (T*)dx, sums);
-            E2A_CHECK_LAUNCH();
-            return sums ? sum_parts(sums, grid, W, dgamma, dbeta, st) : E2A_OK;
-          });
-        });
-      });
-    }
-    k_ln_bwd2<T><<<grid_rows(rows), kThreads, 0, st>>>((const T*)x, ldx, (const T*)dy, lddy, (const T*)u, ldu, n, mean,
-                                                       rstd, rows, (T*)d_dy, (T*)dx, row_u, row_c);
-    E2A_CHECK_LAUNCH();
-    if (!dgamma && !dbeta) return E2A_OK;
-    return launch_cols<T>(true, (const T*)x, ldx, (const T*)dy, lddy, (const T*)u, ldu, n, mean, rstd, row_u, row_c,
-                          rows, part, dgamma, dbeta, st);
-  });
+  const E2aLnBwd2 a{x, ldx, dy, lddy, u, ldu, gamma, beta, mean, rstd, p, q, rows, W, act, d_dy, dx, dgamma, dbeta,
+                    part, row_u, row_c, st};
+  return by_type(dtype, [&](auto* t) { return e2a_ln_bwd2<std::remove_pointer_t<decltype(t)>>(a); });
 }
 
 }  // extern "C"
+#endif
