@@ -371,9 +371,9 @@ struct Shape {
   // vectors of a thread that are never beyond the row's end: by_shape takes every shape but the narrowest (a single
   // vector, or four single values in a team of 8) for rows that fill more than half of it
   static constexpr int SURE = VEC == 1 && TEAM == 8 ? 0 : V / 2;
-  // those of them that are loaded and stored without asking (150,000 x 262 fp32 second order 275 -> 243 us; with 16-byte
-  // vectors the registers fall worse: 16,384 x 4,096 bf16 157 -> 230 us)
-  static constexpr int UNASKED = VEC == 1 ? SURE : 0;
+  // those of them that are loaded and stored without asking (150,000 x 262 fp32 second order 275 -> 243 us, 8,192 x 8,192
+  // bf16 454 -> 388 us; in narrower shapes of 16-byte vectors the registers fall worse: 16,384 x 4,096 bf16 157 -> 230 us)
+  static constexpr int UNASKED = VEC == 1 || TEAM == 512 ? SURE : 0;
   static constexpr int SCRATCH = TEAM > 32 ? 2 * 5 * (TEAM / 32) : 1;                    // team_sum
 };
 
@@ -879,6 +879,7 @@ int64_t most_parts(int64_t rows, int64_t W) {
 // CTAs of a row kernel: as many as the device holds at once, never more than there are batches of rows.
 template <auto Kernel, class S>
 int row_grid(int64_t rows, int64_t W, int* grid) {
+  if (W < S::TEAM * S::VEC * S::SURE) return E2A_ERR_ARG;      // what Shape says of by_shape
   static std::atomic<int> resident_on[64];
   int dev = 0;
   E2A_CUDA(cudaGetDevice(&dev));
