@@ -182,3 +182,42 @@ def test_state_is_not_made_inside_a_capture(bits, when):
     for t in (1, 2):
         graph.replay()
         assert int(opt.state[ps[0]]["step"]) == t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("how", ["clear", "entry", "load", "swap"])
+def test_a_captured_step_stays_good_when_the_state_is_laid_out_again(bits, how):
+    """The state of the same parameters keeps its memory: replays go on from what it was set to."""
+    ps, opt = _pair([300, 300, 20], bits)
+    qs, eager = _pair([300, 300, 20], bits)
+    opt.flat_state()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    graph.replay()
+    for _ in range(2):
+        eager.step()
+    at = {k: t.data_ptr() for k, t in opt.flat_state().items()}
+    for o, ts in ((opt, ps), (eager, qs)):
+        if how == "clear":
+            o.state.clear()
+        elif how == "entry":
+            o.state[ts[1]] = {}
+        elif how == "swap":
+            o.state[ts[0]], o.state[ts[1]] = o.state[ts[1]], o.state[ts[0]]
+        else:
+            saved = copy.deepcopy(o.state_dict())
+            o.step() if o is eager else graph.replay()
+            o.load_state_dict(saved)
+        held = o.flat_state()
+        assert not (how == "clear" and any(bool(t.any()) for t in held.values()))
+        if o is opt:
+            assert at == {k: t.data_ptr() for k, t in held.items()}
+    graph.replay()
+    eager.step()
+    for p, q in zip(ps, qs):
+        assert torch.equal(p, q)
+        for k in eager.state[q]:
+            assert torch.equal(opt.state[p][k], eager.state[q][k]), k

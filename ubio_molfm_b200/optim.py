@@ -151,6 +151,8 @@ class _Flat:
                 self.buffers[k] = torch.zeros(end // BLOCK, dtype=torch.uint8, device=self.device)
         self.entries = [self.view(i, p) for i, p in enumerate(self.params)]
         self.values = [tuple(e.values()) for e in self.entries]
+        self.names = tuple(self.entries[0]) if self.entries else ()
+        self.filled = self.stale = False
 
     def view(self, i, param):
         """The state of tensor ``i``: views of the flat buffers."""
@@ -165,20 +167,35 @@ class _Flat:
     def belongs_to(self, params):
         return len(params) == len(self.params) and all(map(is_, params, self.params))
 
+    def fits(self, params):
+        return self.belongs_to(params) and all(p.numel() == n and p.device == self.device
+                                               for p, n in zip(params, self.numel))
+
     def held_in(self, state):
         """Whether an optimiser's ``state`` has this state's views, and nothing else, for its parameters."""
         return all(state.get(p) is e and len(e) == len(v) and all(map(is_, e.values(), v))
                    for p, e, v in zip(self.params, self.entries, self.values))
 
-    def take(self, i, entry):
-        """Copies a state of tensor ``i`` from elsewhere."""
-        mine = self.entries[i]
-        if set(entry) != set(mine) or any(t.shape != mine[k].shape or (t.dtype != mine[k].dtype and k != "step")
-                                          for k, t in entry.items()):
-            raise ValueError(f"the state of a parameter of shape {list(self.params[i].shape)} is not one of "
-                             f"{self.bits}-bit moments")
-        for k, t in entry.items():
-            mine[k].copy_(t)
+    def fill(self, given):
+        """Takes the states ``given`` for its tensors, where None zeros; what are its own views already stays.  Nothing
+        is changed where one does not fit."""
+        names = self.names
+        for p, e, v in zip(self.params, given, self.values):
+            if e is not None and (set(e) != set(names) or any(
+                    e[k].shape != t.shape or (e[k].dtype != t.dtype and k != "step") for k, t in zip(names, v))):
+                raise ValueError(f"the state of a parameter of shape {list(p.shape)} is not one of {self.bits}-bit moments")
+        # copies first: a given tensor can be a view of another's place
+        moved = [(t, e[k].clone()) for e, v in zip(given, self.values) if e is not None
+                 for k, t in zip(names, v) if e[k] is not t]
+        if self.filled:
+            zeros = self.buffers.values() if not any(given) else [t for e, v in zip(given, self.values) if e is None
+                                                                  for t in v]
+            for t in zeros:
+                t.zero_()
+        for t, value in moved:
+            t.copy_(value)
+        self.entries = [dict(zip(names, v)) for v in self.values]
+        self.filled, self.stale = True, False
 
 
 # group options that change PyTorch's AdamW or this one's arguments, with the only value that they may have here
@@ -214,7 +231,8 @@ class AdamW(torch.optim.Optimizer):
     (``step``, ``exp_avg``, ``exp_avg_sq`` and, in 8 bits, their ``_scale``) are views of one flat buffer per
     group (:meth:`flat_state`); ``state_dict`` / ``load_state_dict`` keep types and bits.  As with PyTorch's, the
     state belongs to the parameter: one that replaces another, or whose entry in ``state`` was cleared, starts anew,
-    and groups may be reordered, shortened or removed between steps (the next step then lays their state out again)."""
+    and groups may be reordered, shortened or removed between steps (the next step then lays their state out again, in
+    the same memory while a group's parameters are the same, so that a captured step goes on from there)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
                  max_grad_norm=None):
@@ -246,10 +264,12 @@ class AdamW(torch.optim.Optimizer):
 
     # -- state -------------------------------------------------------------------------------------
     def _sync(self):
-        """Drops the layouts that ``state`` no longer is the views of, whoever changed it; what it holds is laid out
-        again where a group needs it."""
+        """Marks the layouts that ``state`` no longer is the views of, whoever changed it; what it holds is laid out again
+        where a group needs it."""
         if _lib.load_torch().e2a_state_is_held(self.state, self._held, len(self._held)):
-            self._flat = {i: f for i, f in self._flat.items() if i < len(self.param_groups) and f.held_in(self.state)}
+            self._flat = {i: f for i, f in self._flat.items() if i < len(self.param_groups)}
+            for f in self._flat.values():
+                f.stale = f.stale or not f.held_in(self.state)
             self._hold()
 
     def _hold(self):
@@ -260,19 +280,20 @@ class AdamW(torch.optim.Optimizer):
     def _group_state(self, i):
         self._sync()
         flat, params = self._flat.get(i), self.param_groups[i]["params"]
-        return flat if flat is not None and flat.belongs_to(params) else self._lay_out(i)
+        return flat if flat is not None and not flat.stale and flat.belongs_to(params) else self._lay_out(i)
 
     def _lay_out(self, i):
-        """A flat state for group ``i``, with what ``state`` has for its parameters and zeros for the others."""
+        """A flat state for group ``i``, with what ``state`` has for its parameters and zeros for the others; in the
+        memory of the one that it has where the parameters are the same, so that captured steps stay good."""
         params = self.param_groups[i]["params"]
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW's state would be made inside a graph capture, and made anew by every replay: call "
                                "flat_state() for each group before it")
-        flat = _Flat(params, self.state_bits)
+        flat = self._flat.get(i)
+        if flat is None or not flat.fits(params):
+            flat = _Flat(params, self.state_bits)
         with torch.no_grad():
-            for k, p in enumerate(params):
-                if self.state.get(p):
-                    flat.take(k, self.state[p])
+            flat.fill([self.state.get(p) or None for p in params])
         self.state.update(zip(params, flat.entries))
         self._flat[i] = flat
         self._hold()
@@ -316,7 +337,11 @@ class AdamW(torch.optim.Optimizer):
                       "exp_avg_sq_scale": scales}
             if i in held and any(t.shape != shapes[k] for k, t in held[i].items()):
                 raise ValueError(f"state of parameter {i} has another shape than the parameter's")
+        flats = self._flat
         super().load_state_dict({"state": {}, "param_groups": groups})    # checks and takes the groups
+        self._flat = flats
+        for f in flats.values():
+            f.stale = True
         for gi, (g, mine) in enumerate(zip(groups, self.param_groups)):
             if any(i in held for i in g["params"]):
                 self.state.update((p, held[i]) for i, p in zip(g["params"], mine["params"]) if i in held)
@@ -370,7 +395,7 @@ class AdamW(torch.optim.Optimizer):
         if not params:
             return []
         flat = self._flat.get(gi)
-        if flat is None:
+        if flat is None or flat.stale:
             if all(p.grad is None for p in params):
                 return []
             flat = self._lay_out(gi)
