@@ -13,8 +13,8 @@
 //
 // All of it is bound by memory once the arithmetic is packed and the exponential the special function unit's: the
 // forward moves 2 values an element, the backward 3, the second order 5.  640,210 x 128 fp32 (328 MB an operand):
-// 100, 161 and 243 us, that is 6.5, 6.1 and 6.7 TB/s where a copy runs at 6.5; 97,865 x 512 fp32: 65 and 93 us;
-// 16,384 x 4,096 bf16 without activation: 49 and 82 us (5.5 and 4.9 TB/s: one row a CTA, its sums behind barriers).
+// 102, 164 and 244 us, that is 6.4, 6.0 and 6.7 TB/s where a copy runs at 6.5; 97,865 x 512 fp32: 66 and 94 us;
+// 16,384 x 4,096 bf16 without activation: 49 and 83 us (5.4 and 4.9 TB/s: one row a CTA, its sums behind barriers).
 //
 // The statistics are two-pass in fp32, of the differences to the row's first value, and kept per row.  Column sums: a thread's own rows in fp32 chains of at most
 // 128, which join the CTA's partial rows in memory; those are added up in CTA order in 64 bits.  No atomics.  Rows
@@ -44,7 +44,7 @@ template <> __device__ __forceinline__ __half from_f<__half>(float v) { return _
 // SiLU and its first two derivatives: s = 1 / (1 + exp(-z)), y = z s, y' = s (1 + z (1 - s)),
 // y'' = s (1 - s) (2 + z (1 - 2 s)).  Without activation 1 and 0.  The exponential and the reciprocal are the
 // special function unit's (s within about 2e-7): with expf and a division the forward was bound by them, 212 us
-// on 640,210 x 128 fp32 where copying its bytes takes 109, and is at 110 like this.
+// on 640,210 x 128 fp32 where its bytes take 100, and is at 102 like this.
 struct Act { float y, d1, d2; };
 __device__ __forceinline__ Act activation(float z, bool silu) {
   if (!silu) return {z, 1.f, 0.f};
@@ -855,7 +855,7 @@ int by_shape(int64_t W, bool vec, F f) {
   if (W <= 128) return f(Shape<T, 1, 4, 32>{});
   if (W <= 256) return f(Shape<T, 1, 8, 32>{});
   // 8 values a thread at most beyond a warp, too, where their gradients' sums are held (150,000 x 262 fp32 backward: 519
-  // us with 16, 124 us), 16 in the forward (75 us, 96 us with 8)
+  // us with 16, 117 us), 16 in the forward (71 us; 75 us where 8 took 96)
   if constexpr (WIDE > 16) {
     if (W <= 512) return f(Shape<T, 1, 16, 32>{});
     if (W <= 1024) return f(Shape<T, 1, 16, 64>{});

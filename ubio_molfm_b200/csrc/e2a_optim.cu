@@ -21,8 +21,8 @@
 // The moments' operations are single rounded fp32 ones in a fixed order, so the codes are reproducible bit for bit.
 //
 // With 32-bit moments it is bound by memory: 24.5M fp32 parameters in 240 tensors (28 bytes each) take 99 us, 6.9 TB/s.
-// With 8-bit ones (16 bytes) 84 us where the bytes take 60; 120M bf16 parameters (10 bytes) 345 us where they take 184:
-// 62 instructions an element keep the integer pipe two thirds busy.  The clipping norm of the 24.5M takes 21 to 27 us.
+// With 8-bit ones (16 bytes) 82 us where the bytes take 60; 120M bf16 parameters (10 bytes) 318 us where they take 184:
+// 66 instructions an element keep the integer pipe two thirds busy.  The clipping norm of the 24.5M takes 21 to 27 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -288,7 +288,7 @@ __device__ __forceinline__ uint32_t top_bytes(const uint32_t* w) {
 }
 
 // The step of a whole block of ordinary values, in about half of block_exact's instructions (its time is theirs: 82
-// an element took 408 us on 120M bf16 values, 62 take 345): packed fp32 arithmetic, scales as one product,
+// an element took 408 us on 120M bf16 values, 66 take 318): packed fp32 arithmetic, scales as one product,
 // and square roots within 2^-23.  A root's code is the exact one's unless the rounding offset brings it
 // within a few units of the next code; where that, or a value's range, is in doubt for any of the warp, `sure` is
 // false and the codes are not to be used.  The parameters are stored either way.
